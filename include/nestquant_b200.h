@@ -307,6 +307,52 @@ int nq_ep_barrier(int32_t* const* peer_flags, int rank, int world, int32_t* epoc
  * plus the indexed add of an expert-parallel prefill. */
 int nq_ep_combine(float* out, const void* const* peer_parts, const int32_t* rows, int T, int H, int world, void* stream);
 
+/* ---- around the routed experts ----------------------------------------------------------------------------------
+ * The router's choice, rows sorted by expert and back, and products with plain 4-bit weights.  No counterparts in the reference, whose layer
+ * takes sel and rw from the serving engine and leaves shared experts to it.  Element types: */
+enum { NQ_F32 = 0, NQ_F16 = 1, NQ_BF16 = 2 };
+
+/* sel int64 / rw [T][topk] (what nq_moe_forward and nq_prefill take) from router logits [T][row_stride >= E] of `type`, E <= 1024, topk <= 32.
+ * Chosen are the topk experts with the largest sigmoid(logit) + bias (bias fp32 [E]), or the largest logits if bias is NULL; in falling order,
+ * equal ones by the lowest id; with a bias as the sums are in 64 bits, whatever their roundings to 32.  Experts whose logit or bias is NaN or -inf are
+ * never chosen: where fewer than topk are left, the last ids are -1 and their weights 0.  Weights: scale * p, or scale * p / sum of the chosen p if
+ * renorm, p = sigmoid(logit) (score 0) or the softmax over all experts (score 1, no bias).  One launch. */
+int nq_route(const void* logits, int type, long long row_stride, const float* bias, int T, int E, int topk, int score, int renorm, float scale,
+             int64_t* sel, void* rw, int rw_type, void* stream);
+/* dlogits [T][E] (of `type`, contiguous, all of it written) from drw [T][topk]: the gradient of the weights of nq_route's picks sel.  Choice and bias
+ * have none. */
+int nq_route_bwd(const void* logits, int type, long long row_stride, const int64_t* sel, const void* drw, int rw_type, int T, int E, int topk, int score,
+                 int renorm, float scale, void* dlogits, void* stream);
+
+/* The sort of nq_pf_sort by expert id alone: bin E has the picks whose id is outside [0, E).  start [E + 2]; scratch int32
+ * [nq_pf_sort_scratch_ints(T * topk, E)]. */
+int nq_sort_picks(const int64_t* sel, int T, int topk, int E, int32_t* pe, int32_t* pt, int32_t* pos, int32_t* start, int32_t* scratch, int scratch_ints,
+                  void* stream);
+/* xs[pos[t][k]] = x[t] for picks in front of *live (= start + E of nq_sort_picks), zeros for those behind: all of xs [T * topk][H] is written.
+ * x [T][row_stride >= H].  nq_dispatch_bwd: dx[t] = sum of dxs[pos[t][k]] over the picks in front of *live (32-bit sums, pick order). */
+int nq_dispatch(const void* x, int type, long long row_stride, const int32_t* pos, const int32_t* live, int T, int topk, int H, void* xs, void* stream);
+int nq_dispatch_bwd(const void* dxs, int type, const int32_t* pos, const int32_t* live, int T, int topk, int H, void* dx, void* stream);
+/* out[t] = sum over the picks in front of *live of rw[t][k] y[pos[t][k]] (32-bit sums, pick order; y's other rows are not read).  out_type: type or
+ * NQ_F32.  nq_combine_bwd: dy[pos[t][k]] = rw[t][k] dout[t] (zeros from *live on), drw[t][k] = <y[pos[t][k]], dout[t]> (0 there); dout is of out_type, dy
+ * of type, drw of rw_type; dy or drw may be NULL. */
+int nq_combine(const void* y, int type, const void* rw, int rw_type, const int32_t* pos, const int32_t* live, int T, int topk, int H, void* out, int out_type,
+               void* stream);
+int nq_combine_bwd(const void* dout, int out_type, const void* y, int type, const void* rw, int rw_type, const int32_t* pos, const int32_t* live, int T, int topk,
+                   int H, void* dy, void* drw, void* stream);
+
+/* Matrices of 4-bit weights: (q[n][k] - z[n][k / group]) * s[n][k / group], group 32, 64 or 128, a divisor of K.
+ *   nq_w4_units   number of units (16 rows x 128 columns) of E matrices N x K
+ *   nq_w4_layout  q uint8 [E][N][K / 2] (two columns a byte, the even one in the low half), scales [E][N][K / group] of any 16-bit type, zeros uint8
+ *                 [E][N][K / group] (0 to 15) or NULL (8) -> planes qw [units][1024] bytes, sc [units][16 * 128 / group] 16-bit, zp likewise bytes (NULL
+ *                 without zeros), in the order of nq_w4.cu
+ *   nq_w4_matmul  out[r] = W x[r] for x [rows][x_stride >= K] of `type` (NQ_F16 or NQ_BF16; rows start on 16 bytes), out [rows][out_stride >= N] of type
+ *                 or NQ_F32.  start NULL: one matrix (E = 1) for all rows.  Else int32 [E + 1] on the device: matrix e for the rows start[e] to
+ *                 start[e + 1] - 1 (start[0] = 0), zeros into the rows from start[E] on. */
+int nq_w4_units(int E, int N, int K, int64_t* units);
+int nq_w4_layout(const void* q, const void* scales, const void* zeros, int E, int N, int K, int group, void* qw, void* sc, void* zp, void* stream);
+int nq_w4_matmul(const void* x, int type, long long x_stride, const void* qw, const void* sc, int sc_type, const void* zp, const int32_t* start, int rows, int E,
+                 int N, int K, int group, void* out, int out_type, long long out_stride, void* stream);
+
 /* ---- promotion engine (host side) -------------------------------------------------------------------------------
  * One engine per GPU process, reading that process's record file (fixed-size records, see nestquant_b200/p4rec.py).
  * Replaces the torch-extension class Engine of streaming/nqstream.cu:46-283 (upgrade / post / poll / cancel /

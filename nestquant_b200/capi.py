@@ -13,6 +13,7 @@ NQ_OK, NQ_ERR_ARG, NQ_ERR_CUDA, NQ_ERR_UNSUPPORTED = 0, -1, -2, -3
 TABLE_WIDTH = 20
 MAX_TOKENS = 32
 MAX_PICKS = 256
+NQ_F32, NQ_F16, NQ_BF16 = 0, 1, 2
 
 _p, _i, _i64, _sz = C.c_void_p, C.c_int, C.c_int64, C.c_size_t
 
@@ -88,6 +89,16 @@ SIGNATURES = {
     "nq_moe_static_scratch_bytes": (_sz, []),
     "nq_moe_forward_static": (_i, [_p, _p, _p, _p, _p] + [_i] * 9 + [_p, _p]),
     "nq_salience": (_i, [_p, _i, _i64, _p, _p, _i, _i, _i, _i, C.c_float, _p, _p, _p]),
+    "nq_route": (_i, [_p, _i, _i64, _p, _i, _i, _i, _i, _i, C.c_float, _p, _p, _i, _p]),
+    "nq_route_bwd": (_i, [_p, _i, _i64, _p, _p, _i, _i, _i, _i, _i, _i, C.c_float, _p, _p]),
+    "nq_sort_picks": (_i, [_p, _i, _i, _i, _p, _p, _p, _p, _p, _i, _p]),
+    "nq_dispatch": (_i, [_p, _i, _i64, _p, _p, _i, _i, _i, _p, _p]),
+    "nq_dispatch_bwd": (_i, [_p, _i, _p, _p, _i, _i, _i, _p, _p]),
+    "nq_combine": (_i, [_p, _i, _p, _i, _p, _p, _i, _i, _i, _p, _i, _p]),
+    "nq_combine_bwd": (_i, [_p, _i, _p, _i, _p, _i, _p, _p, _i, _i, _i, _p, _p, _p]),
+    "nq_w4_units": (_i, [_i, _i, _i, C.POINTER(_i64)]),
+    "nq_w4_layout": (_i, [_p, _p, _p, _i, _i, _i, _i, _p, _p, _p, _p]),
+    "nq_w4_matmul": (_i, [_p, _i, _i64, _p, _p, _i, _p, _p, _i, _i, _i, _i, _i, _p, _i, _i64, _p]),
     "nq_ep_barrier": (_i, [C.POINTER(_p), _i, _i, _p, _p, C.c_longlong, _p]),
     "nq_ep_picks": (_i, [C.POINTER(_p), C.POINTER(_p), _i, _i, _i, _i, _i, _p, _p, _p]),
     "nq_ep_gather": (_i, [_p, C.POINTER(_p), _p, _p, _i, _i, _i, _i, _i, _i, _p]),
@@ -143,3 +154,19 @@ def ptr(t):
 def current_stream():
     import torch
     return torch.cuda.current_stream().cuda_stream
+
+
+def element_types():
+    """torch dtype -> NQ_F32 / NQ_F16 / NQ_BF16"""
+    import torch
+    return {torch.float32: NQ_F32, torch.float16: NQ_F16, torch.bfloat16: NQ_BF16}
+
+
+def on_device(t, call, *a):
+    """call(stream) with t's device as the current one and that device's current stream"""
+    import torch
+    d = t.get_device()
+    if d == torch.cuda.current_device():
+        return call(torch.cuda.current_stream(d).cuda_stream, *a)
+    with torch.cuda.device(d):
+        return call(torch.cuda.current_stream(d).cuda_stream, *a)

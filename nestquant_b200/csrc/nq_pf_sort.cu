@@ -4,7 +4,8 @@
 // Replaces the host side of the reference's prefill (sm120/moe.py:293-298: torch.argsort of the flattened expert ids,
 // scatter_add for the counts, a .cpu() of the counts) and this library's earlier use of the same torch operators.
 //   bins     expert id 0 .. E - 1, plus bin E for the picks that contribute nothing (id outside [0, E), expert not resident
-//            on this GPU, routing weight 0): they sort behind every real pair and no kernel touches their rows.
+//            on this GPU, routing weight 0): they sort behind every real pair and no kernel touches their rows.  nq_sort_picks, the
+//            sort around experts that this library does not hold, goes by the ids alone: a weight of 0 still has a gradient.
 //   slices   a warp owns up to 256 consecutive picks.  Pass 1 counts its picks per bin; pass 2 turns the counts into the
 //            offset of every (slice, bin) and the size of every bin; pass 3 walks the slice again, 32 picks at a time in pick
 //            order, and places each pick at start[bin] + offset[slice][bin] + its rank among the slice's earlier picks of that
@@ -34,9 +35,9 @@ __device__ __forceinline__ int pick_bin(const int64_t* sel, const __half* rw, co
                                         int E, int i, bool* hit)
 {
     const int64_t e = sel[i];
-    const bool valid = e >= 0 && e < E && __half2float(rw[i]) != 0.f;
+    const bool valid = e >= 0 && e < E && (!rw || __half2float(rw[i]) != 0.f);
     *hit = valid;
-    return valid && table[e * kTableWidth] > 0 ? (int)e : E;
+    return valid && (!table || table[e * kTableWidth] > 0) ? (int)e : E;
 }
 
 // pass 1: hist[slice][bin] (and hits[e] += picks with a weight)
@@ -214,7 +215,7 @@ int sort_pairs(const int64_t* sel, const void* rw, const int64_t* table, int T, 
     NQ_REQUIRE(start, "nq_pf_sort: null start array");
     cudaStream_t st = (cudaStream_t)stream;
     if (P == 0) return cudaMemsetAsync(start, 0, sizeof(int32_t) * (E + 2), st) == cudaSuccess ? NQ_OK : fail(NQ_ERR_CUDA, "nq_pf_sort: memset failed");
-    NQ_REQUIRE(sel && rw && table && pe && pt && pos && scratch, "nq_pf_sort: null pointer");
+    NQ_REQUIRE(sel && !rw == !table && pe && pt && pos && scratch, "nq_pf_sort: null pointer");
     NQ_REQUIRE(scratch_ints >= nq_pf_sort_scratch_ints(P, E), "nq_pf_sort: scratch needs %d ints", nq_pf_sort_scratch_ints(P, E));
     const size_t small = sizeof(int) * (33 * (size_t)(E + 1) + 1);
     if (P <= kSortSmallPicks && small <= kSortSmallShared)
@@ -248,7 +249,14 @@ int nq_pf_sort_scratch_ints(int pairs, int E)
 int nq_pf_sort(const int64_t* sel, const void* rw, const int64_t* table, int T, int topk, int E, int32_t* pe, int32_t* pt, int32_t* pos,
                int32_t* start, int32_t* hits, int32_t* scratch, int scratch_ints, void* stream)
 {
+    NQ_REQUIRE((rw && table) || T == 0, "nq_pf_sort: null pointer");
     return nq::sort_pairs(sel, rw, table, T, topk, E, pe, pt, pos, start, hits, scratch, scratch_ints, nullptr, 4, stream);
+}
+
+int nq_sort_picks(const int64_t* sel, int T, int topk, int E, int32_t* pe, int32_t* pt, int32_t* pos, int32_t* start, int32_t* scratch, int scratch_ints,
+                  void* stream)
+{
+    return nq::sort_pairs(sel, nullptr, nullptr, T, topk, E, pe, pt, pos, start, nullptr, scratch, scratch_ints, nullptr, 4, stream);
 }
 
 }  // extern "C"
