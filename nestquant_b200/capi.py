@@ -162,11 +162,14 @@ def element_types():
     return {torch.float32: NQ_F32, torch.float16: NQ_F16, torch.bfloat16: NQ_BF16}
 
 
-def on_device(t, call, *a):
-    """call(stream) with t's device as the current one and that device's current stream"""
+def launch(what, f, t, *args):
+    """f(*args, stream), an entry point whose last argument is the stream, on t's device and that device's current stream"""
     import torch
     d = t.get_device()
     if d == torch.cuda.current_device():
-        return call(torch.cuda.current_stream(d).cuda_stream, *a)
-    with torch.cuda.device(d):
-        return call(torch.cuda.current_stream(d).cuda_stream, *a)
+        rc = f(*args, torch._C._cuda_getCurrentRawStream(d))
+    else:
+        with torch.cuda.device(d):
+            rc = f(*args, torch._C._cuda_getCurrentRawStream(d))
+    if rc:
+        check(rc, what)

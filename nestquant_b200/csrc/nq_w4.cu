@@ -12,18 +12,25 @@
 //
 // q - z is exact in fp16 and in bf16 (integers to 15 in magnitude), products and sums of a group are in 32 bits on the tensor pipe, and
 // the group's scale is applied to its sum in 32 bits: nothing is rounded to fewer bits before the result.
+#include <atomic>
+#include <type_traits>
+
 #include "nq_common.cuh"
+#include "nq_scan.cuh"
 #include "nq_types.cuh"
 
 namespace nq {
 
-constexpr int kW4Warps = 8, kW4Tiles = 4, kW4Rows = 8 * kW4Tiles;       // rows of x in a pass
+constexpr int kW4Warps = 16, kW4MaxExperts = 1024;
+constexpr int kW4MaxShared = 216 * 1024;      // planes, rows of x and partial sums, beside the experts' rows
+constexpr int kW4MaxColumns = 32768;          // eight rows of x in a cluster of eight: 66 KB
 
 struct W4 {
     const uint4* qw; const uint16_t* sc; const uint8_t* zp;
     const void* x; const int* start; void* out;
     long long x_stride, out_stride;
-    int rows, N, K, E, S, C, out_type, sc_bf16;
+    int rows, N, K, E, S, C, out_type;
+    int log_ck, log_wk, pitch, blocks, sms;         // see w4_kernel
 };
 
 // ---- layout -------------------------------------------------------------------------------------------------------------------
@@ -65,27 +72,43 @@ __global__ void __launch_bounds__(256) w4_layout_kernel(W4Layout a)
 
 // ---- product ------------------------------------------------------------------------------------------------------------------
 
+// c = a b, or c += a b: a sum that starts does not need zeros in registers
+#define NQ_W4_MMA(T)                                                                                                                               \
+    if (FIRST)                                                                                                                                     \
+        asm("mma.sync.aligned.m16n8k16.row.col.f32." T "." T ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"                      \
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));            \
+    else                                                                                                                                           \
+        asm("mma.sync.aligned.m16n8k16.row.col.f32." T "." T ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"                          \
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1))
+// (w & MASK) | bits, in one instruction
+template <uint32_t MASK>
+__device__ __forceinline__ uint32_t masked(uint32_t w, uint32_t bits)
+{
+    uint32_t v;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(v) : "r"(w), "n"(MASK), "r"(bits));
+    return v;
+}
 template <class X> struct Operand;
 template <> struct Operand<__half> {
+    template <bool FIRST>
     static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
     {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        NQ_W4_MMA("f16");
     }
-    // what is subtracted from the words of the two rows: 1024 + z and 64 + z
-    static __device__ __forceinline__ void zeros(int z0, int z1, uint32_t& lo, uint32_t& hi)
+    // what comes off the words of the two rows (z: their zero points, a byte each): 1024 + z, whose last bit is 1, and -(64 + z), whose last bit is 1 / 16
+    static __device__ __forceinline__ void zeros(uint32_t z, uint32_t& lo, uint32_t& hi)
     {
-        const __half2 a = __half2half2(__int2half_rn(1024 + z0)), b = __half2half2(__int2half_rn(-64 - z1));
-        lo = *reinterpret_cast<const uint32_t*>(&a); hi = *reinterpret_cast<const uint32_t*>(&b);
+        lo = __byte_perm(z, 0x64u, 0x4040);
+        hi = __byte_perm(z >> 4, 0xd4u, 0x4040);      // (z's low byte is below 16)
     }
     // A fragment of a step: 0x6400 | n = 1024 + n, 0x6400 | n << 4 = 1024 + 16 n
     static __device__ __forceinline__ void weights(uint32_t w, uint32_t lo, uint32_t hi, uint32_t (&a)[4])
     {
         const uint32_t w8 = w >> 8, sixteenth = 0x2c002c00u;
-        a[0] = (w & 0x000f000fu) | 0x64006400u;
-        a[1] = (w & 0x00f000f0u) | 0x64006400u;
-        a[2] = (w8 & 0x000f000fu) | 0x64006400u;
-        a[3] = (w8 & 0x00f000f0u) | 0x64006400u;
+        a[0] = masked<0x000f000fu>(w, 0x64006400u);
+        a[1] = masked<0x00f000f0u>(w, 0x64006400u);
+        a[2] = masked<0x000f000fu>(w8, 0x64006400u);
+        a[3] = masked<0x00f000f0u>(w8, 0x64006400u);
         asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(a[0]) : "r"(lo));
         asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(a[1]) : "r"(sixteenth), "r"(hi));
         asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(a[2]) : "r"(lo));
@@ -93,133 +116,465 @@ template <> struct Operand<__half> {
     }
 };
 template <> struct Operand<__nv_bfloat16> {
+    template <bool FIRST>
     static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
     {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        NQ_W4_MMA("bf16");
     }
-    static __device__ __forceinline__ void zeros(int z0, int z1, uint32_t& lo, uint32_t& hi)
+    static __device__ __forceinline__ void zeros(uint32_t z, uint32_t& lo, uint32_t& hi)
     {
-        lo = (0x4300u | z0) * 0x10001u;                   // 128 + z: seven bits of mantissa hold it
-        hi = (0x4300u | z1) * 0x10001u;
+        lo = __byte_perm(z, 0x43u, 0x4040);               // 128 + z: seven bits of mantissa hold it
+        hi = __byte_perm(z, 0x43u, 0x4141);
     }
     static __device__ __forceinline__ void weights(uint32_t w, uint32_t lo, uint32_t hi, uint32_t (&a)[4])
     {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
         {
-            a[i] = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+            a[i] = masked<0x000f000fu>(w >> (4 * i), 0x43004300u);
             asm("sub.rn.bf16x2 %0, %0, %1;" : "+r"(a[i]) : "r"(i & 1 ? hi : lo));
         }
     }
 };
 
-__device__ __forceinline__ float scale_of(uint32_t bits, bool bf16)
+// the two scales in a word
+template <class SC>
+__device__ __forceinline__ float2 scales_of(uint32_t w)
 {
-    return bf16 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half((unsigned short)bits));
+    if (std::is_same<SC, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
-// a strip of 16 rows of one expert's matrix per CTA, the units of its rows split over the warps.  GROUPS: of a unit (1, 2, 4)
-template <class X, int GROUPS>
-__global__ void __launch_bounds__(32 * kW4Warps) w4_kernel(W4 a)
+__device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+// (by 32-bit address: pointers that are moved along lose what space they point to)
+__device__ __forceinline__ uint4 load_shared16(uint32_t at)
 {
-    __shared__ float s_part[kW4Warps][kW4Rows][17];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-    const int strip = blockIdx.x, e = blockIdx.y;
-    int r0 = 0, r1 = a.rows;
-    if (a.start)
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+template <int WORDS>
+__device__ __forceinline__ void load_shared(uint32_t at, uint32_t (&v)[WORDS])
+{
+    if (WORDS == 1) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[0]) : "r"(at));
+    else if (WORDS == 2) asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[1 % WORDS]) : "r"(at));
+    else asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1 % WORDS]), "=r"(v[2 % WORDS]), "=r"(v[3 % WORDS]) : "r"(at));
+}
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from)
+{
+    if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(to), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" :: "r"(to), "l"(from), "n"(BYTES) : "memory");
+}
+template <int LEFT>
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_group %0;" :: "n"(LEFT) : "memory"); }
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
+template <int GROUPS>
+struct W4Unit {
+    uint4 w[2];
+    uint32_t sc[GROUPS];
+    uint32_t zp[(GROUPS + 1) / 2];       // two bytes a group
+};
+// A warp's units on their way through shared memory, kDepth of them asked for ahead.  A lane copies what it reads itself, so nothing but its own
+// copies has to be waited for.
+template <int GROUPS, int DEPTH>
+struct W4Stream {
+    static constexpr int kDepth = DEPTH, kZeroBytes = GROUPS == 4 ? 8 : 4;
+    static constexpr int kScales = 1024, kZeros = kScales + 128 * GROUPS, kStage = kZeros + 32 * kZeroBytes, kBytes = kDepth * kStage;
+    const char *w, *sc, *zp;             // of the next unit to ask for
+    uint32_t place, last;                // of the oldest unit, of the last place
+    int at_w, at_sc, at_zp;              // this lane's, in a place
+    int shift;                           // of this lane's two zero points in their word
+    __device__ __forceinline__ W4Stream(const char* shared, int lane)
+        : place(shared_address(shared)), at_w(lane * 16), at_sc(kScales + lane * 4 * GROUPS), at_zp(kZeros + lane * kZeroBytes), shift(GROUPS == 1 && (lane & 4) ? 16 : 0)
     {
-        // (whatever is in start, rows stay inside x and out)
-        r0 = e == 0 ? 0 : min(max(a.start[e], 0), a.rows);
-        r1 = e == a.E ? a.rows : min(max(a.start[e + 1], r0), a.rows);
+        last = place + (kDepth - 1) * kStage;
     }
-    if (e == a.E)
+    // goes on with the units from `unit` on
+    __device__ __forceinline__ void seek(const W4& a, size_t unit, int lane)
     {
+        w = (const char*)a.qw + unit * 1024 + lane * 16;
+        sc = (const char*)a.sc + (unit * 8 + (lane >> 2)) * 4 * GROUPS;
+        // (one group's two bytes: the aligned word that has them)
+        if (a.zp) zp = (const char*)a.zp + (GROUPS == 1 ? unit * 16 + (lane >> 3) * 4 : (unit * 8 + (lane >> 2)) * 2 * GROUPS);
+    }
+    // asks for the next unit, into the oldest one's place; without one too: the copies are counted
+    __device__ __forceinline__ void ask(bool there, bool zeros)
+    {
+        if (there)
+        {
+            copy_async<16>(place + at_w, w);
+            copy_async<16>(place + at_w + 512, w + 512);
+            copy_async<4 * GROUPS>(place + at_sc, sc);
+            w += 1024; sc += 32 * GROUPS;
+            if (zeros) { copy_async<kZeroBytes>(place + at_zp, zp); zp += 16 * GROUPS; }
+        }
+        copies_end();
+        place = place == last ? last - (kDepth - 1) * kStage : place + kStage;
+    }
+    __device__ __forceinline__ void oldest(W4Unit<GROUPS>& u, bool zeros) const
+    {
+        copies_done<kDepth - 1>();
+        u.w[0] = load_shared16(place + at_w);
+        u.w[1] = load_shared16(place + at_w + 512);
+        load_shared(place + at_sc, u.sc);
+#pragma unroll
+        for (int j = 0; j < (GROUPS + 1) / 2; ++j) u.zp[j] = 0x08080808u;
+        if (zeros)
+        {
+            load_shared(place + at_zp, u.zp);
+            if (GROUPS == 1) u.zp[0] >>= shift;
+        }
+    }
+};
+
+// acc += the unit's 16 x 128 weights times rows of x: xs[n] = shared address of the lane's row of tile n at the unit's columns 8 t
+template <class X, class SC, int GROUPS, int TILES>
+__device__ __forceinline__ void unit_product(const W4Unit<GROUPS>& u, const uint32_t (&xs)[TILES], float (&acc)[TILES][4])
+{
+    const uint32_t words[8] = {u.w[0].x, u.w[0].y, u.w[0].z, u.w[0].w, u.w[1].x, u.w[1].y, u.w[1].z, u.w[1].w};
+#pragma unroll
+    for (int j = 0; j < GROUPS; ++j)
+    {
+        uint32_t lo, hi;
+        Operand<X>::zeros(u.zp[j / 2] >> (16 * (j & 1)), lo, hi);
+        float part[TILES][4];
+#pragma unroll
+        for (int q = 0; q < 4 / GROUPS; ++q)
+        {
+            const int G = j * (4 / GROUPS) + q;
+            uint32_t a0[4], a1[4];
+            Operand<X>::weights(words[2 * G], lo, hi, a0);
+            Operand<X>::weights(words[2 * G + 1], lo, hi, a1);
+#pragma unroll
+            for (int n = 0; n < TILES; ++n)
+            {
+                const uint4 b = load_shared16(xs[n] + G * 64);
+                if (q == 0) Operand<X>::template mma<true>(part[n], a0, b.x, b.y);
+                else Operand<X>::template mma<false>(part[n], a0, b.x, b.y);
+                Operand<X>::template mma<false>(part[n], a1, b.z, b.w);
+            }
+        }
+        const float2 sc = scales_of<SC>(u.sc[j]);
+#pragma unroll
+        for (int n = 0; n < TILES; ++n)
+        {
+            acc[n][0] += sc.x * part[n][0]; acc[n][1] += sc.x * part[n][1];
+            acc[n][2] += sc.y * part[n][2]; acc[n][3] += sc.y * part[n][3];
+        }
+    }
+}
+
+// every thread of every CTA of the cluster arrives and waits
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t cluster_address(uint32_t address, int rank)
+{
+    uint32_t there;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(address), "r"(rank));
+    return there;
+}
+__device__ __forceinline__ void cluster_store(uint32_t address, float x, float y)
+{
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" :: "r"(address), "f"(x), "f"(y) : "memory");
+}
+
+// shared memory of a CTA
+template <int GROUPS, int TILES>
+struct W4Plan {
+    using Stream = W4Stream<GROUPS, TILES == 4 ? 3 : 4>;
+    static constexpr int kPitch = 8 * TILES + 2, kPart = kW4Warps * 16 * kPitch;
+    static constexpr int kPlanes = kW4Warps * Stream::kBytes, kParts = 2 * kPart * 4, kRoom = kW4MaxShared - kPlanes - kParts;      // for rows of x
+};
+
+// An item: a block of strips times the rows of one pass over an expert's rows.  Items are in this order: experts, their passes, blocks.
+struct W4Cursor {
+    int e, pass, block;                  // pass: counted over all experts
+    __device__ __forceinline__ void find(const int* s_first, int E)
+    {
+        int above = E;                   // s_first[e] <= pass < s_first[above], experts without a pass share their successor's
+        while (above - e > 1)
+        {
+            const int m = (e + above) >> 1;
+            if (s_first[m] <= pass) e = m;
+            else above = m;
+        }
+    }
+    __device__ __forceinline__ void seek(int item, int blocks, const int* s_first, int E)
+    {
+        pass = item / blocks; block = item % blocks; e = 0;
+        find(s_first, E);
+    }
+    __device__ __forceinline__ void next(int blocks, const int* s_first, int E, int passes)
+    {
+        if (++block < blocks) return;
+        block = 0;
+        if (++pass < passes && s_first[e + 1] <= pass) find(s_first, E);
+    }
+};
+
+// A warp's share of an item: its part of the columns of one strip times the item's rows, while it asks for what comes kDepth units later
+template <class X, class SC, int GROUPS, int TILES, int MOST, class STREAM, class NEXT>
+__device__ __forceinline__ void strip_product(STREAM& planes, int units, bool zeros, uint32_t x0, int pitch, int rows, int lane,
+                                              float (&acc)[MOST][4], NEXT&& ask)
+{
+    // columns of a tile behind the last row read that row again: nobody looks at what comes of them
+    uint32_t xs[TILES];
+#pragma unroll
+    for (int n = 0; n < TILES; ++n) xs[n] = x0 + min(8 * n + (lane >> 2), rows - 1) * pitch + (lane & 3) * 16;
+    float sum[TILES][4] = {};
+    for (int u = 0; u < units; ++u)
+    {
+        W4Unit<GROUPS> unit;
+        planes.oldest(unit, zeros);
+        unit_product<X, SC, GROUPS, TILES>(unit, xs, sum);
+#pragma unroll
+        for (int n = 0; n < TILES; ++n) xs[n] += 256;
+        ask();
+    }
+#pragma unroll
+    for (int n = 0; n < TILES; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[n][i] = sum[n][i];
+}
+
+// One CTA per SM, in clusters of `ck` that split the matrix into ranges of columns, each taking a run of consecutive items.  A block has ws = 16 / wk strips, wk
+// warps for each: part p = rank wk + warp % wk of parts = ck wk multiplies the units [p C / parts, (p + 1) C / parts) of its strip with up to 8 TILES rows
+// of x, which stay in shared memory as long as the rows are the same.  Units are asked for across the borders of items, so that memory does not
+// wait for sums.  Each CTA of a cluster adds up ws 16 / ck rows of the result: the warps store their parts of those into its shared memory, one
+// barrier per item, whose sums are taken after the next item's products.  The parts are added in their order; how many there are follows from the
+// matrices alone, so a row's bits do not depend on the other rows of the call.
+template <class X, class SC, int GROUPS, int TILES>
+__global__ void __launch_bounds__(32 * kW4Warps, 1) w4_kernel(W4 a)
+{
+    using Plan = W4Plan<GROUPS, TILES>;
+    using Stream = typename Plan::Stream;
+    constexpr int kRows = 8 * TILES, kPitch = Plan::kPitch;
+    // [warp] Stream; [2][part][row of the matrix][row of x] of this CTA's rows, for two items; rows of x, a.pitch apart
+    extern __shared__ __align__(16) char s_planes[];
+    __shared__ int s_row[kW4MaxExperts + 1], s_first[kW4MaxExperts + 2], s_warp[32];       // experts' rows of x, first passes
+    float* const s_part = reinterpret_cast<float*>(s_planes + Plan::kPlanes);
+    char* const s_x = s_planes + Plan::kPlanes + Plan::kParts;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int ck = 1 << a.log_ck, wk = 1 << a.log_wk, ws = kW4Warps >> a.log_wk, log_parts = a.log_ck + a.log_wk, blocks = a.blocks;
+    const int rank = blockIdx.x & (ck - 1), w = warp & (wk - 1), in_block = warp >> a.log_wk, p = (rank << a.log_wk) + w;
+    const int u0 = (p * a.C) >> log_parts, units = (((p + 1) * a.C) >> log_parts) - u0;
+    const int c0 = (rank * a.C) >> a.log_ck, c1 = ((rank + 1) * a.C) >> a.log_ck;      // units of the CTA's rows of x
+    const bool zeros = a.zp != nullptr;
+    int passes;
+    if (!a.start)
+    {
+        passes = (a.rows + kRows - 1) / kRows;
+        if (threadIdx.x == 0) { s_row[0] = s_first[0] = 0; s_row[1] = a.rows; s_first[1] = passes; }
+        __syncthreads();
+    }
+    else
+    {
+        grid_dependency_wait();
+        // two experts a thread; whatever is in start, rows stay inside x and out
+        auto at = [&](int e) { return e == 0 ? 0 : min(max(a.start[min(e, a.E)], 0), a.rows); };
+        const int e0 = 2 * threadIdx.x, x0 = at(e0), x1 = at(e0 + 1), x2 = at(e0 + 2);
+        const int n0 = (max(x1 - x0, 0) + kRows - 1) / kRows, n1 = (max(x2 - x1, 0) + kRows - 1) / kRows;
+        const int before = cta_exclusive_sum(n0 + n1, s_warp, passes);
+        if (threadIdx.x == 0) { s_first[a.E] = passes; s_row[a.E] = at(a.E); }
+        if (e0 < a.E) s_first[e0] = before;
+        if (e0 + 1 < a.E) s_first[e0 + 1] = before + n0;
+        if (e0 < a.E) s_row[e0] = x0;
+        if (e0 + 1 < a.E) s_row[e0 + 1] = x1;
+        __syncthreads();
         // rows behind the last expert's
-        for (int i = threadIdx.x; i < (r1 - r0) * 16; i += blockDim.x)
-            if (strip * 16 + i % 16 < a.N) store_as(a.out, a.out_type, (size_t)(r0 + i / 16) * a.out_stride + strip * 16 + i % 16, 0.f);
+        const int behind = s_row[a.E];
+        for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < (size_t)(a.rows - behind) * a.N; i += (size_t)gridDim.x * blockDim.x)
+            store_as(a.out, a.out_type, (behind + i / a.N) * a.out_stride + i % a.N, 0.f);
+    }
+    // as many items for each cluster, one more for the first ones
+    const unsigned items = (unsigned)passes * blocks, clusters = gridDim.x >> a.log_ck, mine = blockIdx.x >> a.log_ck, each = items / clusters, more = items % clusters;
+    const int i0 = mine * each + min(mine, more), i1 = i0 + each + (mine < more);
+    if (i0 == i1)                                         // the whole cluster
+    {
+        if (!a.start) grid_dependency_wait();
+        launch_dependents();
         return;
     }
-    const size_t unit0 = ((size_t)e * a.S + strip) * a.C;
-    for (int base = r0; base < r1; base += kW4Rows)
+    Stream planes(s_planes + warp * Stream::kBytes, lane);
+    W4Cursor now, ahead;
+    now.seek(i0, blocks, s_first, a.E);
+    ahead = now;
+    int to_ask = i1 - i0, in_strip = 0;      // items to ask for, units left of the present one
+    bool there = true;
+    auto ask = [&] {
+        if (--in_strip < 0)
+        {
+            if (to_ask-- > 0)
+            {
+                // (strips behind the last one: that one again, nobody looks at what comes of it)
+                planes.seek(a, ((size_t)ahead.e * a.S + min(ahead.block * ws + in_block, a.S - 1)) * a.C + u0, lane);
+                ahead.next(blocks, s_first, a.E, passes);
+                in_strip = units - 1;
+            }
+            else { there = false; in_strip = 0x7fffffff; }
+        }
+        planes.ask(there, zeros);
+    };
+    // the planes do not come from a kernel that lets its successors in early: those of a single matrix are asked for before the wait
+#pragma unroll 1
+    for (int d = 0; d < Stream::kDepth; ++d) ask();
+    if (!a.start) grid_dependency_wait();
+    launch_dependents();
+    if (ck > 1) cluster_arrive();                       // the others' shared memory is there when all have come by
+    const int log_own = 8 - a.log_wk - a.log_ck, own = 1 << log_own;       // rows of the matrix whose sums this CTA adds up: ws 16 / ck
+    // the sums of an item whose parts have been stored, after the barrier
+    auto add_up = [&](const float* part, int block, int base, int rows) {
+        for (int i = threadIdx.x; i < rows * own; i += blockDim.x)
+        {
+            const int r = i >> log_own, n = i & (own - 1), to = block * ws * 16 + rank * own + n;
+            float sum = 0.f;
+#pragma unroll 8
+            for (int q = 0; q < 1 << log_parts; ++q) sum += part[((q << log_own) + n) * kPitch + r];
+            if (to < a.N) store_as(a.out, a.out_type, (size_t)(base + r) * a.out_stride + to, sum);
+        }
+    };
+    auto barrier = [&] {
+        if (ck > 1) cluster_wait();
+        else __syncthreads();
+    };
+    int old_block = -1, old_base = 0, old_rows = 0, pass = -1, base = 0, rows = 0;
+    for (int i = i0; i < i1; ++i)
     {
-        float acc[kW4Tiles][4] = {};
-        for (int c = warp; c < a.C; c += kW4Warps)
+        if (now.pass != pass)
         {
-            const size_t unit = unit0 + c;
-            uint4 w[2];
-            w[0] = a.qw[unit * 64 + lane];
-            w[1] = a.qw[unit * 64 + 32 + lane];
-            const uint32_t* words = reinterpret_cast<const uint32_t*>(w);
-#pragma unroll
-            for (int j = 0; j < GROUPS; ++j)
+            // other rows of x: pieces of 256 columns, in turn to the warps
+            pass = now.pass;
+            base = s_row[now.e] + (pass - s_first[now.e]) * kRows;
+            rows = min(max(s_row[now.e + 1], s_row[now.e]) - base, kRows);
+            __syncthreads();
+            const int pieces = (c1 - c0 + 1) / 2;
+            for (int r = 0, c = warp; r < rows; c += kW4Warps)
             {
-                const size_t at = unit * 16 * GROUPS + (g * GROUPS + j) * 2;
-                const uint32_t s2 = *reinterpret_cast<const uint32_t*>(a.sc + at);
-                int z0 = 8, z1 = 8;
-                if (a.zp) { z0 = a.zp[at]; z1 = a.zp[at + 1]; }
-                uint32_t lo, hi;
-                Operand<X>::zeros(z0, z1, lo, hi);
-                float part[kW4Tiles][4] = {};
-#pragma unroll
-                for (int q = 0; q < 4 / GROUPS; ++q)
-                {
-                    const int G = j * (4 / GROUPS) + q, k = c * 128 + G * 32 + 8 * t;
-                    uint32_t a0[4], a1[4];
-                    Operand<X>::weights(words[2 * G], lo, hi, a0);
-                    Operand<X>::weights(words[2 * G + 1], lo, hi, a1);
-#pragma unroll
-                    for (int n = 0; n < kW4Tiles; ++n)
-                    {
-                        const int r = base + 8 * n + g;
-                        uint4 b = {};
-                        if (r < r1 && k < a.K) b = *reinterpret_cast<const uint4*>((const X*)a.x + r * a.x_stride + k);
-                        Operand<X>::mma(part[n], a0, b.x, b.y);
-                        Operand<X>::mma(part[n], a1, b.z, b.w);
-                    }
-                }
-                const float s0 = scale_of(s2 & 0xffffu, a.sc_bf16), s1 = scale_of(s2 >> 16, a.sc_bf16);
-#pragma unroll
-                for (int n = 0; n < kW4Tiles; ++n)
-                {
-                    acc[n][0] += s0 * part[n][0]; acc[n][1] += s0 * part[n][1];
-                    acc[n][2] += s1 * part[n][2]; acc[n][3] += s1 * part[n][3];
-                }
+                while (c >= pieces) { c -= pieces; ++r; }
+                const int k = (c0 + 2 * c) * 128 + lane * 8, there = k < a.K ? 16 : 0;       // zeros behind the last column
+                if (r < rows && k < c1 * 128)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(shared_address(s_x) + r * a.pitch + (2 * c * 128 + lane * 8) * 2),
+                                 "l"((const X*)a.x + (size_t)(base + r) * a.x_stride + (there ? k : 0)), "r"(there) : "memory");
             }
+            copies_end();
+            copies_done<0>();                             // (and the units that were asked for before)
+            __syncthreads();
         }
+        const uint32_t x0 = shared_address(s_x) + (u0 - c0) * 256;
+        float acc[TILES][4];
+        if (TILES >= 2 && rows <= 8) strip_product<X, SC, GROUPS, 1>(planes, units, zeros, x0, a.pitch, rows, lane, acc, ask);
+        else if (TILES == 4 && rows <= 16) strip_product<X, SC, GROUPS, 2>(planes, units, zeros, x0, a.pitch, rows, lane, acc, ask);
+        else strip_product<X, SC, GROUPS, TILES>(planes, units, zeros, x0, a.pitch, rows, lane, acc, ask);
+        // the item before this one: all its parts are there, and those of the one before that have been read
+        if (i > i0 || ck > 1) barrier();
+        if (i > i0) add_up(s_part + ((i - 1) & 1) * Plan::kPart, old_block, old_base, old_rows);
+        const uint32_t to = shared_address(s_part + (i & 1) * Plan::kPart);
 #pragma unroll
-        for (int n = 0; n < kW4Tiles; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s_part[warp][8 * n + 2 * t + (i & 1)][g + 8 * (i >> 1)] = acc[n][i];
-        __syncthreads();
-        for (int i = threadIdx.x; i < kW4Rows * 16; i += blockDim.x)
+        for (int h = 0; h < 2; ++h)
         {
-            const int r = i / 16, n = i % 16;
-            if (base + r < r1 && strip * 16 + n < a.N)
-            {
-                float sum = 0.f;
+            const int n = in_block * 16 + 8 * h + g, owner = n >> log_own;
+            const uint32_t at = cluster_address(to + (((p << log_own) + (n & (own - 1))) * kPitch + 2 * t) * 4, owner);
 #pragma unroll
-                for (int w = 0; w < kW4Warps; ++w) sum += s_part[w][r][n];
-                store_as(a.out, a.out_type, (size_t)(base + r) * a.out_stride + strip * 16 + n, sum);
-            }
+            for (int q = 0; q < TILES; ++q)
+                if (q == 0 || 8 * q < rows) cluster_store(at + 32 * q, acc[q][2 * h], acc[q][2 * h + 1]);
         }
-        __syncthreads();
+        if (ck > 1) cluster_arrive();
+        old_block = now.block; old_base = base; old_rows = rows;
+        now.next(blocks, s_first, a.E, passes);
     }
+    barrier();
+    add_up(s_part + ((i1 - 1) & 1) * Plan::kPart, old_block, old_base, old_rows);
 }
 
 bool w4_shape(int E, int N, int K, int g)
 {
-    return E >= 1 && E <= 65534 && N >= 1 && (g == 32 || g == 64 || g == 128) && K >= g && K % g == 0;
+    return E >= 1 && E <= kW4MaxExperts && N >= 1 && K <= kW4MaxColumns && (g == 32 || g == 64 || g == 128) && K >= g && K % g == 0;
 }
 int w4_strips(int N) { return (N - 1) / 16 + 1; }
 int w4_chunks(int K) { return (K - 1) / 128 + 1; }
 
-template <class X>
-void w4_launch(const W4& a, int g, dim3 grid, cudaStream_t st)
+// Parts that a strip's columns are cut into: as few units per warp as the device's warps allow, two more for each item's sums.  Goes by the
+// matrices, not by the rows of a call; of several experts eight are taken to have rows.  And no more than 1,024 columns a part: 32 rows of x
+// beside one another in shared memory.
+int w4_parts(int S, int C, int E, int sms)
 {
-    if (g == 128) w4_kernel<X, 1><<<grid, 32 * kW4Warps, 0, st>>>(a);
-    else if (g == 64) w4_kernel<X, 2><<<grid, 32 * kW4Warps, 0, st>>>(a);
-    else w4_kernel<X, 4><<<grid, 32 * kW4Warps, 0, st>>>(a);
+    const long long strips = (long long)S * (E < 8 ? E : 8), warps = (long long)sms * kW4Warps;
+    int best = 1;
+    long long cost = -1;
+    for (int parts = 1; parts <= 64 && parts <= C; parts *= 2)
+    {
+        const long long c = ((strips * parts + warps - 1) / warps) * ((C + parts - 1) / parts + 2);
+        if (cost < 0 || c < cost) { cost = c; best = parts; }
+    }
+    while (best < (C + 7) / 8 && 2 * best <= 64 && 2 * best <= C) best *= 2;
+    return best;
+}
+
+// bytes between rows of x in shared memory: 64 off a multiple of 128, so that two rows of a fragment share the banks
+int w4_pitch(int C, int ck) { return ((C + ck - 1) / ck) * 256 + 64; }
+
+// clusters of ck CTAs that the device runs at a time, one CTA per SM
+template <class K>
+int w4_clusters(K* kernel, int ck, int sms, int device, cudaLaunchConfig_t& cfg)
+{
+    static std::atomic<int> known[16][4];
+    if (ck == 1) return sms;
+    std::atomic<int>* const at = device < 16 ? &known[device][ck == 2 ? 0 : ck == 4 ? 1 : 2] : nullptr;
+    int n = at ? at->load(std::memory_order_relaxed) : 0;
+    if (n) return n;
+    cfg.gridDim = dim3(ck);
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) { cudaGetLastError(); n = 1; }
+    if (at) at->store(n, std::memory_order_relaxed);
+    return n;
+}
+
+template <class X, class SC, int GROUPS, int TILES>
+int w4_launch(W4 a, int parts, int device, cudaStream_t st)
+{
+    using Plan = W4Plan<GROUPS, TILES>;
+    const int rows = a.rows < 8 * TILES ? a.rows : 8 * TILES;
+    // as few CTAs share a strip as the room for rows of x allows
+    int ck = 1;
+    while (ck < 8 && ck < parts && (parts / ck > kW4Warps || rows * w4_pitch(a.C, ck) > Plan::kRoom)) ck *= 2;
+    const int ws = kW4Warps / (parts / ck);
+    for (a.log_ck = 0; 1 << a.log_ck < ck; ++a.log_ck) {}
+    for (a.log_wk = 0; ck << a.log_wk < parts; ++a.log_wk) {}
+    a.pitch = w4_pitch(a.C, ck);
+    a.blocks = (a.S + ws - 1) / ws;
+    const long long most = (long long)a.blocks * (a.start ? a.rows / (8 * TILES) + (a.E < a.rows ? a.E : a.rows) : (a.rows - 1) / (8 * TILES) + 1);
+    NQ_REQUIRE(most <= 0x7fffffff / a.C, "nq_w4_matmul: %d rows are too many", a.rows);       // (units are counted in 32 bits)
+    auto* kernel = w4_kernel<X, SC, GROUPS, TILES>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(32 * kW4Warps); cfg.dynamicSmemBytes = Plan::kPlanes + Plan::kParts + (size_t)rows * a.pitch; cfg.stream = st;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kW4MaxShared) != cudaSuccess) return fail(NQ_ERR_CUDA, "nq_w4_matmul: shared memory");
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ck; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = 1;
+    long long clusters = w4_clusters(kernel, ck, a.sms, device, cfg);
+    if (most < clusters) clusters = most;
+    cfg.gridDim = dim3((unsigned)(clusters * ck));
+    cfg.numAttrs = 2;
+    cudaLaunchKernelEx(&cfg, kernel, a);
+    return check_launch("nq_w4_matmul");
+}
+template <class X, class SC, int GROUPS>
+int w4_tiles(const W4& a, int device, cudaStream_t st)
+{
+    // as many tiles of eight rows as the call has, up to four; fewer where shared memory does not hold that many rows
+    const int parts = w4_parts(a.S, a.C, a.E, a.sms), pitch = w4_pitch(a.C, parts < 8 ? parts : 8);
+    if (a.rows <= 8 || 16 * pitch > W4Plan<GROUPS, 2>::kRoom) return w4_launch<X, SC, GROUPS, 1>(a, parts, device, st);
+    if (a.rows <= 16 || 32 * pitch > W4Plan<GROUPS, 4>::kRoom) return w4_launch<X, SC, GROUPS, 2>(a, parts, device, st);
+    return w4_launch<X, SC, GROUPS, 4>(a, parts, device, st);
+}
+template <class X, class SC>
+int w4_groups(const W4& a, int g, int device, cudaStream_t st)
+{
+    return g == 128 ? w4_tiles<X, SC, 1>(a, device, st) : g == 64 ? w4_tiles<X, SC, 2>(a, device, st) : w4_tiles<X, SC, 4>(a, device, st);
 }
 
 }  // namespace nq
@@ -256,11 +611,13 @@ int nq_w4_matmul(const void* x, int type, long long x_stride, const void* qw, co
     NQ_REQUIRE(x && qw && sc && out, "nq_w4_matmul: null pointer");
     NQ_REQUIRE(nq::aligned16(x) && x_stride % 8 == 0 && nq::aligned16(qw) && nq::aligned16(sc), "nq_w4_matmul: rows of x and planes start on 16 bytes");
     nq::W4 a{(const uint4*)qw, (const uint16_t*)sc, (const uint8_t*)zp, x, start, out, x_stride, out_stride, rows, N, K, E, nq::w4_strips(N), nq::w4_chunks(K),
-             out_type, sc_type == NQ_BF16};
-    const dim3 grid(a.S, start ? E + 1 : 1);
-    if (type == NQ_F16) nq::w4_launch<__half>(a, group, grid, (cudaStream_t)stream);
-    else nq::w4_launch<__nv_bfloat16>(a, group, grid, (cudaStream_t)stream);
-    return nq::check_launch("nq_w4_matmul");
+             out_type, 0, 0, 0, 0, 0};
+    int device;
+    if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&a.sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
+        return nq::fail(NQ_ERR_CUDA, "nq_w4_matmul: no device");
+    cudaStream_t st = (cudaStream_t)stream;
+    if (type == NQ_F16) return sc_type == NQ_F16 ? nq::w4_groups<__half, __half>(a, group, device, st) : nq::w4_groups<__half, __nv_bfloat16>(a, group, device, st);
+    return sc_type == NQ_F16 ? nq::w4_groups<__nv_bfloat16, __half>(a, group, device, st) : nq::w4_groups<__nv_bfloat16, __nv_bfloat16>(a, group, device, st);
 }
 
 }  // extern "C"

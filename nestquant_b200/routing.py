@@ -13,7 +13,7 @@ on which a leaf's gradient was first accumulated, which a capture forbids.  Erro
 """
 import torch
 
-from .capi import NestQuantError, check, element_types, lib, on_device
+from .capi import NestQuantError, element_types, launch, lib
 
 _TYPE = element_types()
 _SCORES = {"sigmoid": 0, "softmax": 1}
@@ -37,6 +37,11 @@ def _strided(t):
 
 def _stride(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _once(grad):
+    if torch.is_grad_enabled() and grad is not None and grad.requires_grad:
+        raise NestQuantError("gradients of gradients: not built")
 
 
 # ---- route ----------------------------------------------------------------------------------------------------------------------
@@ -74,9 +79,8 @@ def _route(logits, bias, topk, score, renorm, scale, dtype):
     T, E = logits.shape
     sel = torch.empty(T, topk, dtype=torch.int64, device=logits.device)
     rw = torch.empty(T, topk, dtype=dtype, device=logits.device)
-    check(on_device(logits, lambda st: lib().nq_route(
-        logits.data_ptr(), _TYPE[logits.dtype], _stride(logits), bias.data_ptr() if bias is not None else None, T, E, topk, score, renorm, scale,
-        sel.data_ptr(), rw.data_ptr(), _TYPE[dtype], st)), "route")
+    launch("route", lib().nq_route, logits, logits.data_ptr(), _TYPE[logits.dtype], _stride(logits), None if bias is None else bias.data_ptr(), T, E, topk,
+           score, renorm, scale, sel.data_ptr(), rw.data_ptr(), _TYPE[dtype])
     return sel, rw
 
 
@@ -87,19 +91,21 @@ class _Route(torch.autograd.Function):
         ctx.save_for_backward(logits, sel)
         ctx.how = topk, score, renorm, scale
         ctx.mark_non_differentiable(sel)
+        ctx.set_materialize_grads(False)             # (zeros for sel would be a launch)
         return sel, rw
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, _, drw):
+        _once(drw)
+        if drw is None:
+            return (None,) * 7
         logits, sel = ctx.saved_tensors
         topk, score, renorm, scale = ctx.how
         drw = drw.contiguous()
         T, E = logits.shape
         grad = torch.empty(T, E, dtype=logits.dtype, device=logits.device)
-        check(on_device(logits, lambda st: lib().nq_route_bwd(
-            logits.data_ptr(), _TYPE[logits.dtype], _stride(logits), sel.data_ptr(), drw.data_ptr(), _TYPE[drw.dtype], T, E, topk, score, renorm, scale,
-            grad.data_ptr(), st)), "route backward")
+        launch("route backward", lib().nq_route_bwd, logits, logits.data_ptr(), _TYPE[logits.dtype], _stride(logits), sel.data_ptr(), drw.data_ptr(),
+               _TYPE[drw.dtype], T, E, topk, score, renorm, scale, grad.data_ptr())
         return grad, None, None, None, None, None, None
 
 
@@ -138,7 +144,7 @@ def sort_picks(sel, E):
     buf = torch.empty(E + 2 + 3 * P + max(ints, 1), dtype=torch.int32, device=sel.device)       # (the scratch behind the arrays)
     o = Order(T, topk, E, buf)
     at = lambda i: o._pos + 4 * i * P
-    check(on_device(sel, lambda st: lib().nq_sort_picks(sel.data_ptr(), T, topk, E, at(1), at(2), at(0), o._ptr, at(3), max(ints, 1), st)), "sort_picks")
+    launch("sort_picks", lib().nq_sort_picks, sel, sel.data_ptr(), T, topk, E, at(1), at(2), at(0), o._ptr, at(3), max(ints, 1))
     return o
 
 
@@ -159,8 +165,7 @@ def dispatch(x, order):
 def _dispatch(x, order):
     H = x.shape[1]
     xs = torch.empty(order.P, H, dtype=x.dtype, device=x.device)
-    check(on_device(x, lambda st: lib().nq_dispatch(x.data_ptr(), _TYPE[x.dtype], _stride(x), order._pos, order._live, order.T, order.topk, H,
-                                                    xs.data_ptr(), st)), "dispatch")
+    launch("dispatch", lib().nq_dispatch, x, x.data_ptr(), _TYPE[x.dtype], _stride(x), order._pos, order._live, order.T, order.topk, H, xs.data_ptr())
     return xs
 
 
@@ -171,14 +176,13 @@ class _Dispatch(torch.autograd.Function):
         return _dispatch(x, order)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dxs):
+        _once(dxs)
         o = ctx.order
         dxs = dxs.contiguous()
         H = dxs.shape[1]
         dx = torch.empty(o.T, H, dtype=dxs.dtype, device=dxs.device)
-        check(on_device(dxs, lambda st: lib().nq_dispatch_bwd(dxs.data_ptr(), _TYPE[dxs.dtype], o._pos, o._live, o.T, o.topk, H, dx.data_ptr(), st)),
-              "dispatch backward")
+        launch("dispatch backward", lib().nq_dispatch_bwd, dxs, dxs.data_ptr(), _TYPE[dxs.dtype], o._pos, o._live, o.T, o.topk, H, dx.data_ptr())
         return dx, None
 
 
@@ -202,8 +206,8 @@ def combine(y, order, rw, dtype=None):
 def _combine(y, rw, order, dtype):
     H = y.shape[1]
     out = torch.empty(order.T, H, dtype=dtype, device=y.device)
-    check(on_device(y, lambda st: lib().nq_combine(y.data_ptr(), _TYPE[y.dtype], rw.data_ptr(), _TYPE[rw.dtype], order._pos, order._live, order.T, order.topk, H,
-                                                   out.data_ptr(), _TYPE[dtype], st)), "combine")
+    launch("combine", lib().nq_combine, y, y.data_ptr(), _TYPE[y.dtype], rw.data_ptr(), _TYPE[rw.dtype], order._pos, order._live, order.T, order.topk, H,
+           out.data_ptr(), _TYPE[dtype])
     return out
 
 
@@ -215,13 +219,12 @@ class _Combine(torch.autograd.Function):
         return _combine(y, rw, order, dtype)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
+        _once(dout)
         y, rw = ctx.saved_tensors
         o, dout = ctx.order, dout.contiguous()
         dy = torch.empty_like(y) if ctx.needs_input_grad[0] else None
         drw = torch.empty_like(rw) if ctx.needs_input_grad[1] else None
-        check(on_device(y, lambda st: lib().nq_combine_bwd(
-            dout.data_ptr(), _TYPE[dout.dtype], y.data_ptr(), _TYPE[y.dtype], rw.data_ptr(), _TYPE[rw.dtype], o._pos, o._live, o.T, o.topk, y.shape[1],
-            dy.data_ptr() if dy is not None else None, drw.data_ptr() if drw is not None else None, st)), "combine backward")
+        launch("combine backward", lib().nq_combine_bwd, y, dout.data_ptr(), _TYPE[dout.dtype], y.data_ptr(), _TYPE[y.dtype], rw.data_ptr(), _TYPE[rw.dtype],
+               o._pos, o._live, o.T, o.topk, y.shape[1], None if dy is None else dy.data_ptr(), None if drw is None else drw.data_ptr())
         return dy, drw, None, None

@@ -9,7 +9,7 @@ import ctypes as C
 
 import torch
 
-from .capi import NestQuantError, check, element_types, lib, on_device
+from .capi import NestQuantError, check, element_types, launch, lib
 
 _TYPE = element_types()
 _HALVES = (torch.float16, torch.bfloat16)
@@ -56,8 +56,11 @@ class W4:
         s._sc = torch.empty(n.value * per, dtype=scales.dtype, device=q.device)
         s._zp = None if zeros is None else torch.empty(n.value * per, dtype=torch.uint8, device=q.device)
         q, scales, zeros = q.contiguous(), scales.contiguous(), None if zeros is None else zeros.contiguous()
-        check(on_device(q, lambda st: lib().nq_w4_layout(q.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), s.E, s.N, s.K, s.group,
-                                                         s._qw.data_ptr(), s._sc.data_ptr(), None if zeros is None else s._zp.data_ptr(), st)), "W4")
+        # addresses of the planes, for the calls
+        s._planes = s._qw.data_ptr(), s._sc.data_ptr(), _TYPE[scales.dtype], None if zeros is None else s._zp.data_ptr()
+        s._index = q.get_device()
+        launch("W4", lib().nq_w4_layout, q, q.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), s.E, s.N, s.K, s.group,
+               s._planes[0], s._planes[1], s._planes[3])
 
     def nbytes(s):
         """bytes of the planes on the device"""
@@ -67,23 +70,26 @@ class W4:
         if not (isinstance(x, torch.Tensor) and x.is_cuda and x.dim() == 2 and x.dtype in _HALVES):
             raise NestQuantError("W4: x, expected a CUDA tensor [T,K] of torch.float16 / torch.bfloat16")
         T, K = x.shape
-        dtype = dtype or x.dtype
-        if K != s.K or dtype not in (x.dtype, torch.float32):
-            raise NestQuantError(f"W4: x {tuple(x.shape)} of {x.dtype} as {dtype}, a matrix of {s.K} columns (result in x's own type, or fp32)")
-        if x.get_device() != s._qw.get_device():
+        own = x.dtype
+        dtype = dtype or own
+        if K != s.K or dtype is not own and dtype is not torch.float32:
+            raise NestQuantError(f"W4: x {tuple(x.shape)} of {own} as {dtype}, a matrix of {s.K} columns (result in x's own type, or fp32)")
+        if x.get_device() != s._index:
             raise NestQuantError("W4: x and the weights are on different devices")
         if x.requires_grad and torch.is_grad_enabled():
             raise NestQuantError("W4: no gradient (detach x, or call under torch.no_grad)")
         if (s.experts is None) != (start is None):
             raise NestQuantError("W4: start goes with one matrix per expert, and only with that")
         if start is not None and not (isinstance(start, torch.Tensor) and start.is_cuda and start.dtype == torch.int32 and start.is_contiguous() and
-                                      start.numel() > s.E and start.get_device() == x.get_device()):
+                                      start.numel() > s.E and start.get_device() == s._index):
             raise NestQuantError(f"W4: start, expected a contiguous CUDA tensor of torch.int32 [{s.E + 1}]")
-        if T > 1 and (x.stride(0) < K or x.stride(0) % 8) or x.stride(1) != 1 or x.data_ptr() % 16:
-            x = x.clone(memory_format=torch.contiguous_format)      # rows that the kernel reads start on 16 bytes
-        out = torch.empty(T, s.N, dtype=dtype, device=x.device)
-        check(on_device(x, lambda st: lib().nq_w4_matmul(
-            x.data_ptr(), _TYPE[x.dtype], x.stride(0) if T > 1 else K, s._qw.data_ptr(), s._sc.data_ptr(), _TYPE[s._sc.dtype],
-            s._zp.data_ptr() if s._zp is not None else None, start.data_ptr() if start is not None else None, T, s.E, s.N, s.K, s.group, out.data_ptr(),
-            _TYPE[dtype], s.N, st)), "W4")
+        rows, cols = x.stride()
+        if T <= 1:
+            rows = K
+        if cols != 1 or rows < K or rows % 8 or x.data_ptr() % 16:
+            x, rows = x.clone(memory_format=torch.contiguous_format), K      # rows that the kernel reads start on 16 bytes
+        out = torch.empty((T, s.N), dtype=dtype, device=s.device)
+        qw, sc, sc_type, zp = s._planes
+        launch("W4", lib().nq_w4_matmul, x, x.data_ptr(), _TYPE[own], rows, qw, sc, sc_type, zp, None if start is None else start.data_ptr(), T, s.E, s.N, K,
+               s.group, out.data_ptr(), _TYPE[dtype], s.N)
         return out
