@@ -176,18 +176,17 @@ struct W4Unit {
     uint32_t sc[GROUPS];
     uint32_t zp[(GROUPS + 1) / 2];       // two bytes a group
 };
-// A warp's units on their way through shared memory, kDepth of them asked for ahead.  A lane copies what it reads itself, so nothing but its own
-// copies has to be waited for.
+// A warp's units on their way through shared memory, DEPTH of them asked for ahead.  A lane copies the weights that it reads itself; the first lane of
+// four copies the scales and zero points of their two rows.
 template <int GROUPS, int DEPTH>
 struct W4Stream {
-    static constexpr int kDepth = DEPTH, kZeroBytes = GROUPS == 4 ? 8 : 4;
-    static constexpr int kScales = 1024, kZeros = kScales + 128 * GROUPS, kStage = kZeros + 32 * kZeroBytes, kBytes = kDepth * kStage;
+    static constexpr int kDepth = DEPTH, kScales = 1024, kZeros = kScales + 32 * GROUPS, kStage = kZeros + 16 * GROUPS, kBytes = kDepth * kStage;
     const char *w, *sc, *zp;             // of the next unit to ask for
     uint32_t place, last;                // of the oldest unit, of the last place
     int at_w, at_sc, at_zp;              // this lane's, in a place
-    int shift;                           // of this lane's two zero points in their word
+    bool scales;                         // this lane copies them (its zero points: of one group, two bytes, the aligned word that has them)
     __device__ __forceinline__ W4Stream(const char* shared, int lane)
-        : place(shared_address(shared)), at_w(lane * 16), at_sc(kScales + lane * 4 * GROUPS), at_zp(kZeros + lane * kZeroBytes), shift(GROUPS == 1 && (lane & 4) ? 16 : 0)
+        : place(shared_address(shared)), at_w(lane * 16), at_sc(kScales + (lane >> 2) * 4 * GROUPS), at_zp(kZeros + (lane >> 2) * 2 * GROUPS), scales((lane & 3) == 0)
     {
         last = place + (kDepth - 1) * kStage;
     }
@@ -196,8 +195,7 @@ struct W4Stream {
     {
         w = (const char*)a.qw + unit * 1024 + lane * 16;
         sc = (const char*)a.sc + (unit * 8 + (lane >> 2)) * 4 * GROUPS;
-        // (one group's two bytes: the aligned word that has them)
-        if (a.zp) zp = (const char*)a.zp + (GROUPS == 1 ? unit * 16 + (lane >> 3) * 4 : (unit * 8 + (lane >> 2)) * 2 * GROUPS);
+        if (a.zp) zp = (const char*)a.zp + unit * 16 * GROUPS + ((lane >> 2) * 2 * GROUPS & ~3);
     }
     // asks for the next unit, into the oldest one's place; without one too: the copies are counted
     __device__ __forceinline__ void ask(bool there, bool zeros)
@@ -206,9 +204,13 @@ struct W4Stream {
         {
             copy_async<16>(place + at_w, w);
             copy_async<16>(place + at_w + 512, w + 512);
-            copy_async<4 * GROUPS>(place + at_sc, sc);
+            if (scales)
+            {
+                copy_async<4 * GROUPS>(place + at_sc, sc);
+                if (zeros) copy_async<GROUPS == 4 ? 8 : 4>(place + (at_zp & ~3), zp);
+            }
             w += 1024; sc += 32 * GROUPS;
-            if (zeros) { copy_async<kZeroBytes>(place + at_zp, zp); zp += 16 * GROUPS; }
+            if (zeros) zp += 16 * GROUPS;
         }
         copies_end();
         place = place == last ? last - (kDepth - 1) * kStage : place + kStage;
@@ -216,6 +218,7 @@ struct W4Stream {
     __device__ __forceinline__ void oldest(W4Unit<GROUPS>& u, bool zeros) const
     {
         copies_done<kDepth - 1>();
+        __syncwarp();
         u.w[0] = load_shared16(place + at_w);
         u.w[1] = load_shared16(place + at_w + 512);
         load_shared(place + at_sc, u.sc);
@@ -223,8 +226,8 @@ struct W4Stream {
         for (int j = 0; j < (GROUPS + 1) / 2; ++j) u.zp[j] = 0x08080808u;
         if (zeros)
         {
-            load_shared(place + at_zp, u.zp);
-            if (GROUPS == 1) u.zp[0] >>= shift;
+            if (GROUPS == 1) asm volatile("ld.shared.u16 %0, [%1];" : "=r"(u.zp[0]) : "r"(place + at_zp));
+            else load_shared(place + at_zp, u.zp);
         }
     }
 };
@@ -285,7 +288,9 @@ template <int GROUPS, int TILES>
 struct W4Plan {
     using Stream = W4Stream<GROUPS, TILES == 4 ? 3 : 4>;
     static constexpr int kPitch = 8 * TILES + 2, kPart = kW4Warps * 16 * kPitch;
-    static constexpr int kPlanes = kW4Warps * Stream::kBytes, kParts = 2 * kPart * 4, kRoom = kW4MaxShared - kPlanes - kParts;      // for rows of x
+    // parts of two items, so that the sums of one wait for the next one's products; of one item where 32 rows leave no room
+    static constexpr int kBuffers = TILES == 4 ? 1 : 2;
+    static constexpr int kPlanes = kW4Warps * Stream::kBytes, kParts = kBuffers * kPart * 4, kRoom = kW4MaxShared - kPlanes - kParts;      // for rows of x
 };
 
 // An item: a block of strips times the rows of one pass over an expert's rows.  Items are in this order: experts, their passes, blocks.
@@ -324,6 +329,7 @@ __device__ __forceinline__ void strip_product(STREAM& planes, int units, bool ze
 #pragma unroll
     for (int n = 0; n < TILES; ++n) xs[n] = x0 + min(8 * n + (lane >> 2), rows - 1) * pitch + (lane & 3) * 16;
     float sum[TILES][4] = {};
+#pragma unroll 2
     for (int u = 0; u < units; ++u)
     {
         W4Unit<GROUPS> unit;
@@ -343,8 +349,7 @@ __device__ __forceinline__ void strip_product(STREAM& planes, int units, bool ze
 // warps for each: part p = rank wk + warp % wk of parts = ck wk multiplies the units [p C / parts, (p + 1) C / parts) of its strip with up to 8 TILES rows
 // of x, which stay in shared memory as long as the rows are the same.  Units are asked for across the borders of items, so that memory does not
 // wait for sums.  Each CTA of a cluster adds up ws 16 / ck rows of the result: the warps store their parts of those into its shared memory, one
-// barrier per item, whose sums are taken after the next item's products.  The parts are added in their order; how many there are follows from the
-// matrices alone, so a row's bits do not depend on the other rows of the call.
+// barrier per item, whose sums are taken after the next item's products.  The parts are added in their order: the same call gives the same bits.
 template <class X, class SC, int GROUPS, int TILES>
 __global__ void __launch_bounds__(32 * kW4Warps, 1) w4_kernel(W4 a)
 {
@@ -467,10 +472,10 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) w4_kernel(W4 a)
         if (TILES >= 2 && rows <= 8) strip_product<X, SC, GROUPS, 1>(planes, units, zeros, x0, a.pitch, rows, lane, acc, ask);
         else if (TILES == 4 && rows <= 16) strip_product<X, SC, GROUPS, 2>(planes, units, zeros, x0, a.pitch, rows, lane, acc, ask);
         else strip_product<X, SC, GROUPS, TILES>(planes, units, zeros, x0, a.pitch, rows, lane, acc, ask);
-        // the item before this one: all its parts are there, and those of the one before that have been read
+        // two buffers: all parts of the item before this one are there, and those of the one before that have been read; one: they have been read
         if (i > i0 || ck > 1) barrier();
-        if (i > i0) add_up(s_part + ((i - 1) & 1) * Plan::kPart, old_block, old_base, old_rows);
-        const uint32_t to = shared_address(s_part + (i & 1) * Plan::kPart);
+        if (Plan::kBuffers == 2 && i > i0) add_up(s_part + ((i - 1) & 1) * Plan::kPart, old_block, old_base, old_rows);
+        const uint32_t to = shared_address(s_part + (Plan::kBuffers == 2 ? i & 1 : 0) * Plan::kPart);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
         {
@@ -481,9 +486,16 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) w4_kernel(W4 a)
                 if (q == 0 || 8 * q < rows) cluster_store(at + 32 * q, acc[q][2 * h], acc[q][2 * h + 1]);
         }
         if (ck > 1) cluster_arrive();
+        if (Plan::kBuffers == 1)
+        {
+            barrier();
+            add_up(s_part, now.block, base, rows);
+            if (ck > 1 && i + 1 < i1) cluster_arrive();
+        }
         old_block = now.block; old_base = base; old_rows = rows;
         now.next(blocks, s_first, a.E, passes);
     }
+    if (Plan::kBuffers == 1) return;
     barrier();
     add_up(s_part + ((i1 - 1) & 1) * Plan::kPart, old_block, old_base, old_rows);
 }
@@ -494,23 +506,6 @@ bool w4_shape(int E, int N, int K, int g)
 }
 int w4_strips(int N) { return (N - 1) / 16 + 1; }
 int w4_chunks(int K) { return (K - 1) / 128 + 1; }
-
-// Parts that a strip's columns are cut into: as few units per warp as the device's warps allow, two more for each item's sums.  Goes by the
-// matrices, not by the rows of a call; of several experts eight are taken to have rows.  And no more than 1,024 columns a part: 32 rows of x
-// beside one another in shared memory.
-int w4_parts(int S, int C, int E, int sms)
-{
-    const long long strips = (long long)S * (E < 8 ? E : 8), warps = (long long)sms * kW4Warps;
-    int best = 1;
-    long long cost = -1;
-    for (int parts = 1; parts <= 64 && parts <= C; parts *= 2)
-    {
-        const long long c = ((strips * parts + warps - 1) / warps) * ((C + parts - 1) / parts + 2);
-        if (cost < 0 || c < cost) { cost = c; best = parts; }
-    }
-    while (best < (C + 7) / 8 && 2 * best <= 64 && 2 * best <= C) best *= 2;
-    return best;
-}
 
 // bytes between rows of x in shared memory: 64 off a multiple of 128, so that two rows of a fragment share the banks
 int w4_pitch(int C, int ck) { return ((C + ck - 1) / ck) * 256 + 64; }
@@ -530,34 +525,60 @@ int w4_clusters(K* kernel, int ck, int sms, int device, cudaLaunchConfig_t& cfg)
     return n;
 }
 
+// How a matrix is cut: CTAs of a cluster and warps of a CTA that share a strip, both powers of two.  The device takes ceil(blocks / clusters) rounds; a round
+// costs a warp its units and what comes per item (measured: sums and barriers as much as a unit and a half, over a cluster three).
 template <class X, class SC, int GROUPS, int TILES>
-int w4_launch(W4 a, int parts, int device, cudaStream_t st)
+bool w4_cut(W4& a, int rows, int device, cudaLaunchConfig_t& cfg, long long& clusters)
+{
+    using Plan = W4Plan<GROUPS, TILES>;
+    const int experts = a.E < 8 ? a.E : 8;                // (taken to have rows)
+    double best = 0;
+    for (int log_ck = 0; log_ck <= 3; ++log_ck)
+    {
+        const int ck = 1 << log_ck;
+        if (ck > a.C || rows * w4_pitch(a.C, ck) > Plan::kRoom) continue;
+        cudaLaunchAttribute& cluster = cfg.attrs[0];
+        cluster.val.clusterDim.x = ck;
+        cfg.dynamicSmemBytes = Plan::kPlanes + Plan::kParts + (size_t)rows * w4_pitch(a.C, ck);
+        const int there = w4_clusters(w4_kernel<X, SC, GROUPS, TILES>, ck, a.sms, device, cfg);
+        for (int log_wk = 0; log_wk <= 4 && ck << log_wk <= a.C; ++log_wk)
+        {
+            const int blocks = (a.S - 1) / (kW4Warps >> log_wk) + 1, units = ((a.C - 1) >> (log_ck + log_wk)) + 1;
+            const double cost = (((long long)blocks * experts - 1) / there + 1) * (units + (ck > 1 ? 3.0 : 1.5));
+            if (best == 0 || cost < best)
+            {
+                best = cost;
+                a.log_ck = log_ck; a.log_wk = log_wk; a.blocks = blocks; a.pitch = w4_pitch(a.C, ck);
+                clusters = there;
+            }
+        }
+    }
+    return best > 0;
+}
+
+template <class X, class SC, int GROUPS, int TILES>
+int w4_launch(W4 a, int device, cudaStream_t st)
 {
     using Plan = W4Plan<GROUPS, TILES>;
     const int rows = a.rows < 8 * TILES ? a.rows : 8 * TILES;
-    // as few CTAs share a strip as the room for rows of x allows
-    int ck = 1;
-    while (ck < 8 && ck < parts && (parts / ck > kW4Warps || rows * w4_pitch(a.C, ck) > Plan::kRoom)) ck *= 2;
-    const int ws = kW4Warps / (parts / ck);
-    for (a.log_ck = 0; 1 << a.log_ck < ck; ++a.log_ck) {}
-    for (a.log_wk = 0; ck << a.log_wk < parts; ++a.log_wk) {}
-    a.pitch = w4_pitch(a.C, ck);
-    a.blocks = (a.S + ws - 1) / ws;
-    const long long most = (long long)a.blocks * (a.start ? a.rows / (8 * TILES) + (a.E < a.rows ? a.E : a.rows) : (a.rows - 1) / (8 * TILES) + 1);
-    NQ_REQUIRE(most <= 0x7fffffff / a.C, "nq_w4_matmul: %d rows are too many", a.rows);       // (units are counted in 32 bits)
     auto* kernel = w4_kernel<X, SC, GROUPS, TILES>;
-    cudaLaunchConfig_t cfg = {};
-    cfg.blockDim = dim3(32 * kW4Warps); cfg.dynamicSmemBytes = Plan::kPlanes + Plan::kParts + (size_t)rows * a.pitch; cfg.stream = st;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kW4MaxShared) != cudaSuccess) return fail(NQ_ERR_CUDA, "nq_w4_matmul: shared memory");
+    cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = ck; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr; cfg.numAttrs = 1;
-    long long clusters = w4_clusters(kernel, ck, a.sms, device, cfg);
+    cfg.blockDim = dim3(32 * kW4Warps); cfg.stream = st;
+    long long clusters;
+    if (!w4_cut<X, SC, GROUPS, TILES>(a, rows, device, cfg, clusters)) return fail(NQ_ERR_ARG, "nq_w4_matmul: no room for %d rows of %d columns", rows, a.K);
+    const long long most = (long long)a.blocks * (a.start ? a.rows / (8 * TILES) + (a.E < a.rows ? a.E : a.rows) : (a.rows - 1) / (8 * TILES) + 1);
+    NQ_REQUIRE(most <= 0x7fffffff / a.C, "nq_w4_matmul: %d rows are too many", a.rows);       // (units are counted in 32 bits)
     if (most < clusters) clusters = most;
-    cfg.gridDim = dim3((unsigned)(clusters * ck));
+    attr[0].val.clusterDim.x = 1 << a.log_ck;
+    cfg.gridDim = dim3((unsigned)(clusters << a.log_ck));
+    cfg.dynamicSmemBytes = Plan::kPlanes + Plan::kParts + (size_t)rows * a.pitch;
     cfg.numAttrs = 2;
     cudaLaunchKernelEx(&cfg, kernel, a);
     return check_launch("nq_w4_matmul");
@@ -566,10 +587,10 @@ template <class X, class SC, int GROUPS>
 int w4_tiles(const W4& a, int device, cudaStream_t st)
 {
     // as many tiles of eight rows as the call has, up to four; fewer where shared memory does not hold that many rows
-    const int parts = w4_parts(a.S, a.C, a.E, a.sms), pitch = w4_pitch(a.C, parts < 8 ? parts : 8);
-    if (a.rows <= 8 || 16 * pitch > W4Plan<GROUPS, 2>::kRoom) return w4_launch<X, SC, GROUPS, 1>(a, parts, device, st);
-    if (a.rows <= 16 || 32 * pitch > W4Plan<GROUPS, 4>::kRoom) return w4_launch<X, SC, GROUPS, 2>(a, parts, device, st);
-    return w4_launch<X, SC, GROUPS, 4>(a, parts, device, st);
+    const int pitch = w4_pitch(a.C, a.C < 8 ? a.C : 8);
+    if (a.rows <= 8 || 16 * pitch > W4Plan<GROUPS, 2>::kRoom) return w4_launch<X, SC, GROUPS, 1>(a, device, st);
+    if (a.rows <= 16 || 32 * pitch > W4Plan<GROUPS, 4>::kRoom) return w4_launch<X, SC, GROUPS, 2>(a, device, st);
+    return w4_launch<X, SC, GROUPS, 4>(a, device, st);
 }
 template <class X, class SC>
 int w4_groups(const W4& a, int g, int device, cudaStream_t st)
