@@ -98,7 +98,7 @@ SIGNATURES = {
     "nq_combine_bwd": (_i, [_p, _i, _p, _i, _p, _i, _p, _p, _i, _i, _i, _p, _p, _p]),
     "nq_w4_units": (_i, [_i, _i, _i, C.POINTER(_i64)]),
     "nq_w4_layout": (_i, [_p, _p, _p, _i, _i, _i, _i, _p, _p, _p, _p]),
-    "nq_w4_matmul": (_i, [_p, _i, _i64, _p, _p, _i, _p, _p, _i, _i, _i, _i, _i, _p, _i, _i64, _p]),
+    "nq_w4_matmul": (_i, [_p, _i, _i64, _p, _p, _i, _p, _p, _i, _i, _i, _i, _i, _p, _i, _i64, _p, _p]),
     "nq_ep_barrier": (_i, [C.POINTER(_p), _i, _i, _p, _p, C.c_longlong, _p]),
     "nq_ep_picks": (_i, [C.POINTER(_p), C.POINTER(_p), _i, _i, _i, _i, _i, _p, _p, _p]),
     "nq_ep_gather": (_i, [_p, C.POINTER(_p), _p, _p, _i, _i, _i, _i, _i, _i, _p]),

@@ -1,0 +1,444 @@
+// Products with 4-bit weights (nq_w4.cuh) for calls of many rows: on the fifth-generation tensor cores, 128 rows of the matrix times TOKENS rows of x per item.
+//
+//   warps 0..7    sums: each has 32 rows of the matrix (its quarter of tensor memory) and half of the tokens; adds every group's sums, times the
+//                 group's scale, to its registers, and writes the item's results
+//   warps 8..15   weights: each streams one strip of 16 rows (W4Stream), turns a unit into exact halves q - z and stores them as the MMA's A operand
+//                 in tensor memory (16x256b stores take the fragments as they are)
+//   warp 16       TMA: the tokens' tiles [TOKENS x 64], two per chunk of 128 columns
+//   warp 17       one lane issues tcgen05.mma, 128 x TOKENS x 16 a step, into one of two accumulators per group of columns: an accumulator holds one
+//                 group's sum only, so that the scale is applied in 32 bits and nothing is rounded before the result
+// Columns of an item may be split over a cluster; each CTA then adds up a share of the tokens, the others' sums come through distributed shared memory.
+// Every mbarrier wait is bounded (nq_tc.cuh): on time-out the CTA raises status[0], waits for its loads and MMAs in flight and ends.
+#include "nq_tc.cuh"
+#include "nq_w4.cuh"
+
+namespace nq {
+
+constexpr int kWgSumWarps = 8, kWgDecodeWarps = 8, kWgThreads = 32 * (kWgSumWarps + kWgDecodeWarps + 2);
+
+struct WgShared {
+    uint64_t full_a[6], full_b[6], empty[6], sum_full[2], sum_empty[2], done;
+    uint32_t tmem;
+    PfWaits waits;
+    int row[kW4MaxExperts + 1], first[kW4MaxExperts + 2], warp_sums[32];
+};
+template <int GROUPS, int TOKENS>
+struct WgPlan {
+    using Stream = W4Stream<GROUPS, 4>;
+    static constexpr int kStages = TOKENS == 128 ? 4 : 6;                 // chunks ahead; a weight tile is 64 columns of tensor memory
+    static constexpr int kBox = TOKENS * 128;                             // a token tile of 64 columns
+    static constexpr int kTiles = kStages * 2 * kBox, kPlanes = kWgDecodeWarps * Stream::kBytes, kSums = TOKENS * 512;
+    // tiles, and after them, or in their place once they are through, the sums of a split item; planes
+    static constexpr int kRest = kTiles > kSums ? kTiles : kSums, kSmem = kRest + kPlanes + (int)sizeof(WgShared);
+    static_assert(kSmem <= 232448, "shared memory of a CTA");
+};
+
+extern __shared__ __align__(1024) uint8_t wg_smem[];
+
+__device__ __forceinline__ void tma_two_boxes(uint32_t dst, uint32_t box, const CUtensorMap* map, int x, int y, uint32_t bar)
+{
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(2 * box) : "memory");
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst + box), "l"(map), "r"(x + 64), "r"(y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void mma_step(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(saddr(bar)) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16_async(uint32_t taddr, uint32_t (&v)[16])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+                   "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                 : "r"(taddr) : "memory");
+}
+// (the registers pass through the wait: nothing reads them in front of it)
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&v)[16])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]),
+                   "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]) :: "memory");
+}
+
+struct Wg {
+    W4 w;
+    int* status;
+    int log_ck;
+};
+
+// a counter of stages with the parity of their barriers
+template <int N>
+struct Ring {
+    uint32_t s = 0, parity = 0;
+    __device__ __forceinline__ void next() { if (++s == N) { s = 0; parity ^= 1u; } }
+};
+
+template <class X, class SC, int GROUPS, int TOKENS>
+__global__ void __launch_bounds__(kWgThreads, 1) w4_gemm_kernel(const __grid_constant__ CUtensorMap map, Wg g)
+{
+    using Plan = WgPlan<GROUPS, TOKENS>;
+    using Stream = typename Plan::Stream;
+    constexpr int kStages = Plan::kStages;
+    WgShared& sh = *reinterpret_cast<WgShared*>(wg_smem + Plan::kRest + Plan::kPlanes);
+    const W4& a = g.w;
+    uint8_t* const s_planes = wg_smem + Plan::kRest;
+    const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int ck = 1 << g.log_ck, rank = blockIdx.x & (ck - 1);
+    if (saddr(wg_smem) & 1023u)          // (never: the swizzled tiles would be read from the wrong places)
+    {
+        grid_dependency_wait();
+        if (threadIdx.x == 0) atomicExch(g.status, 1);
+        return;
+    }
+    const int c0 = (rank * a.C) >> g.log_ck, c1 = ((rank + 1) * a.C) >> g.log_ck, blocks = a.blocks;
+    const bool zeros = a.zp != nullptr;
+    if (threadIdx.x == 0)
+    {
+        for (int s = 0; s < kStages; ++s) { mbar_init(&sh.full_a[s], kWgDecodeWarps); mbar_init(&sh.full_b[s], 1); mbar_init(&sh.empty[s], 1); }
+        for (int s = 0; s < 2; ++s) { mbar_init(&sh.sum_full[s], 1); mbar_init(&sh.sum_empty[s], kWgSumWarps); }
+        mbar_init(&sh.done, 1);
+        sh.waits.aborted = 0; sh.waits.limit_ns = (unsigned long long)kPfWaitNs;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 17)
+    {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(&sh.tmem)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    int passes;
+    if (!a.start)
+    {
+        passes = (a.rows + TOKENS - 1) / TOKENS;
+        if (threadIdx.x == 0) { sh.row[0] = sh.first[0] = 0; sh.row[1] = a.rows; sh.first[1] = passes; }
+    }
+    else
+    {
+        grid_dependency_wait();
+        passes = expert_passes<TOKENS>(a, sh.row, sh.first, sh.warp_sums);
+        zero_rows_behind(a, sh.row[a.E]);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = uniform(sh.tmem);
+    const unsigned items = (unsigned)passes * blocks, clusters = gridDim.x >> g.log_ck, mine = blockIdx.x >> g.log_ck, each = items / clusters, more = items % clusters;
+    const int i0 = mine * each + min(mine, more), i1 = i0 + each + (mine < more);
+    W4Cursor now;
+    now.seek(i0 < i1 ? i0 : 0, blocks, sh.first, a.E);
+    // rows of x of an item
+    auto rows_of = [&](const W4Cursor& c, int& base) {
+        base = sh.row[c.e] + (c.pass - sh.first[c.e]) * TOKENS;
+        return min(max(sh.row[c.e + 1], sh.row[c.e]) - base, TOKENS);
+    };
+    float sum[TOKENS / 2];                                // of warps 0 to 7
+    int last_base = 0, last_rows = 0, last_block = 0;
+    if (warp < kWgSumWarps)
+    {
+        // ---- sums
+        const int quarter = warp & 3, half = warp >> 2;
+        const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + half * (TOKENS / 2);
+        Ring<2> acc;
+        bool ok = true;
+        for (int i = i0; i < i1 && ok; ++i, now.next(blocks, sh.first, a.E, passes))
+        {
+            int base;
+            const int rows = rows_of(now, base), r = quarter * 32 + lane;
+            const size_t unit = ((size_t)now.e * a.S + min(now.block * 8 + r / 16, a.S - 1)) * a.C;
+            const uint16_t* sc = a.sc + unit * 16 * GROUPS + (r & 7) * 2 * GROUPS + (r >> 3 & 1);
+            // scales two chunks ahead
+            uint16_t next[2][GROUPS];
+#pragma unroll
+            for (int d = 0; d < 2; ++d)
+#pragma unroll
+                for (int j = 0; j < GROUPS; ++j) next[d][j] = c0 + d < c1 ? sc[(size_t)(c0 + d) * 16 * GROUPS + 2 * j] : 0;
+#pragma unroll
+            for (int j = 0; j < TOKENS / 2; ++j) sum[j] = 0.f;
+            for (int c = c0; c < c1 && ok; ++c)
+            {
+                uint16_t scale[GROUPS];
+#pragma unroll
+                for (int j = 0; j < GROUPS; ++j)
+                {
+                    scale[j] = next[0][j];
+                    next[0][j] = next[1][j];
+                    next[1][j] = c + 2 < c1 ? sc[(size_t)(c + 2) * 16 * GROUPS + 2 * j] : 0;
+                }
+#pragma unroll
+                for (int j = 0; j < GROUPS; ++j)
+                {
+                    ok = ok && mbar_wait_warp(saddr(&sh.sum_full[acc.s]), acc.parity, &sh.waits);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const float s = scales_of<SC>(scale[j]).x;
+#pragma unroll
+                    for (int t0 = 0; t0 < TOKENS / 2; t0 += 32)
+                    {
+                        uint32_t v[16], w[16];
+                        constexpr bool kTwo = TOKENS >= 64;
+                        tmem_ld16_async(from + acc.s * TOKENS + t0, v);
+                        if (kTwo) tmem_ld16_async(from + acc.s * TOKENS + t0 + 16, w);
+                        tmem_wait_ld(v);
+                        if (kTwo) tmem_wait_ld(w);
+                        if (t0 + 32 >= TOKENS / 2)
+                        {
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&sh.sum_empty[acc.s]);
+                        }
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) sum[t0 + k] += s * __uint_as_float(v[k]);
+                        if (kTwo)
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) sum[(t0 + 16 + k) % (TOKENS / 2)] += s * __uint_as_float(w[k]);
+                    }
+                    acc.next();
+                }
+            }
+            last_base = base; last_rows = rows; last_block = now.block;
+            if (ck == 1 && ok)
+            {
+                const int n = now.block * 128 + r;
+                if (n < a.N)
+#pragma unroll
+                    for (int t = 0; t < TOKENS / 2; ++t)
+                        if (half * (TOKENS / 2) + t < rows) store_as(a.out, a.out_type, (size_t)(base + half * (TOKENS / 2) + t) * a.out_stride + n, sum[t]);
+            }
+        }
+    }
+    else if (warp < kWgSumWarps + kWgDecodeWarps)
+    {
+        // ---- weights.  A warp reaches the quarter of tensor memory that its number has: strips 2 (warp % 4) and the one behind it
+        const int strip = 2 * (warp & 3) + (warp >> 2 & 1);
+        Stream planes((const char*)s_planes + (warp - kWgSumWarps) * Stream::kBytes, lane);
+        W4Cursor ahead = now;
+        int to_ask = i1 - i0, left = 0;
+        bool there = true;
+        auto ask = [&] {
+            if (--left < 0)
+            {
+                if (to_ask-- > 0)
+                {
+                    planes.seek(a, ((size_t)ahead.e * a.S + min(ahead.block * 8 + strip, a.S - 1)) * a.C + c0, lane);
+                    ahead.next(blocks, sh.first, a.E, passes);
+                    left = c1 - c0 - 1;
+                }
+                else { there = false; left = 0x7fffffff; }
+            }
+            planes.ask(there, zeros);
+        };
+#pragma unroll 1
+        for (int d = 0; d < Stream::kDepth; ++d) ask();
+        const uint32_t to = tmem + ((uint32_t)(strip * 16) << 16) + 2 * TOKENS;
+        Ring<kStages> stage;
+        for (int u = (i1 - i0) * (c1 - c0); u > 0; --u)
+        {
+            W4Unit<GROUPS> unit;
+            planes.oldest(unit, zeros);
+            const uint32_t words[8] = {unit.w[0].x, unit.w[0].y, unit.w[0].z, unit.w[0].w, unit.w[1].x, unit.w[1].y, unit.w[1].z, unit.w[1].w};
+            if (!mbar_wait_warp(saddr(&sh.empty[stage.s]), stage.parity ^ 1u, &sh.waits)) break;
+            tc_fence_after();
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+            {
+                uint32_t r[16];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                {
+                    constexpr int kSteps = 8 / GROUPS;
+                    const int group = (4 * h + j) / kSteps;
+                    uint32_t lo, hi, f[4];
+                    Operand<X>::zeros(unit.zp[group / 2] >> (16 * (group & 1)), lo, hi);
+                    Operand<X>::weights(words[4 * h + j], lo, hi, f);
+                    r[4 * j] = f[0]; r[4 * j + 1] = f[2]; r[4 * j + 2] = f[1]; r[4 * j + 3] = f[3];
+                }
+                tmem_st_16x256b_x4(to + stage.s * 64 + h * 32, r);
+            }
+            ask();
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.full_a[stage.s]);
+            stage.next();
+        }
+        copies_done<0>();
+    }
+    else if (warp == 16)
+    {
+        // ---- token tiles
+        if (!a.start) grid_dependency_wait();
+        const uint32_t tiles = saddr(wg_smem);
+        Ring<kStages> stage;
+        uint32_t asked = 0;                               // bit s: parity of the loads into stage s
+        bool ok = true;
+        for (int i = i0; i < i1 && ok; ++i, now.next(blocks, sh.first, a.E, passes))
+        {
+            int base;
+            rows_of(now, base);
+            for (int c = c0; c < c1; ++c)
+            {
+                ok = mbar_wait_warp(saddr(&sh.empty[stage.s]), stage.parity ^ 1u, &sh.waits);
+                if (!ok) break;
+                if (lane == 0) tma_two_boxes(tiles + stage.s * 2 * Plan::kBox, Plan::kBox, &map, c * 128, base, saddr(&sh.full_b[stage.s]));
+                __syncwarp();
+                asked ^= 1u << stage.s;
+                stage.next();
+            }
+        }
+        for (int s = 0; s < kStages; ++s) mbar_wait_own(saddr(&sh.full_b[s]), ((asked >> s) & 1u) ^ 1u);      // loads on their way
+    }
+    else
+    {
+        // ---- MMAs
+        constexpr uint32_t kType = std::is_same<X, __half>::value ? 0u : 1u;
+        constexpr uint32_t kDesc = (1u << 4) | (kType << 7) | (kType << 10) | ((uint32_t)(TOKENS >> 3) << 17) | (8u << 24);      // fp32 sums, both operands K-major, M 128
+        const uint64_t b0 = smem_desc(saddr(wg_smem), 16, 1024, 2);
+        Ring<kStages> stage;
+        Ring<2> acc;
+        bool ok = true;
+        for (int u = (i1 - i0) * (c1 - c0); u > 0 && ok; --u)
+        {
+            ok = mbar_wait_warp(saddr(&sh.full_a[stage.s]), stage.parity, &sh.waits) && mbar_wait_warp(saddr(&sh.full_b[stage.s]), stage.parity, &sh.waits);
+#pragma unroll
+            for (int j = 0; j < GROUPS; ++j)
+            {
+                ok = ok && mbar_wait_warp(saddr(&sh.sum_empty[acc.s]), acc.parity ^ 1u, &sh.waits);
+                if (!ok) break;
+                tc_fence_after();
+                if (lane == 0)
+                {
+                    const uint32_t d = tmem + acc.s * TOKENS, w = tmem + 2 * TOKENS + stage.s * 64;
+#pragma unroll
+                    for (int q = 0; q < 8 / GROUPS; ++q)
+                    {
+                        const int k = j * (8 / GROUPS) + q;       // step of the chunk
+                        mma_step(d, w + k * 8, b0 + ((stage.s * 2 * Plan::kBox + (k >> 2) * Plan::kBox + (k & 3) * 32) >> 4), kDesc, q != 0);
+                    }
+                    commit(&sh.sum_full[acc.s]);
+                    if (j == GROUPS - 1) commit(&sh.empty[stage.s]);
+                }
+                __syncwarp();
+                acc.next();
+            }
+            stage.next();
+        }
+        if (lane == 0) commit(&sh.done);
+        __syncwarp();
+        mbar_wait_own(saddr(&sh.done), 0);
+    }
+    launch_dependents();
+    if (ck > 1)
+    {
+        // one item: every CTA of the cluster is through with its tiles, whose place takes the sums: [rank][token of this CTA's share][row]
+        tc_fence_before();
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+        const int share = TOKENS >> g.log_ck, log_share = 31 - __clz(share);
+        if (warp < kWgSumWarps && i0 < i1)
+        {
+            const int quarter = warp & 3, half = warp >> 2;
+#pragma unroll
+            for (int t = 0; t < TOKENS / 2; ++t)
+            {
+                const int token = half * (TOKENS / 2) + t;
+                const uint32_t at = cluster_address(saddr(wg_smem) + ((((rank << log_share) + (token & (share - 1))) << 7) + quarter * 32 + lane) * 4, token >> log_share);
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(sum[t]) : "memory");
+            }
+        }
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+        if (i0 < i1)
+        {
+            // (what every thread needs of the item)
+            int base;
+            W4Cursor item;
+            item.seek(i0, blocks, sh.first, a.E);
+            const int rows = rows_of(item, base);
+            const float* part = reinterpret_cast<const float*>(wg_smem);
+            for (int i = threadIdx.x; i < share * 128; i += blockDim.x)
+            {
+                const int token = (rank << log_share) + (i >> 7), n = item.block * 128 + (i & 127);
+                if (token >= rows || n >= a.N) continue;
+                float s = 0.f;
+#pragma unroll 8
+                for (int q = 0; q < ck; ++q) s += part[(q << (log_share + 7)) + i];
+                store_as(a.out, a.out_type, (size_t)(base + token) * a.out_stride + n, s);
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (sh.waits.aborted && threadIdx.x == 0) atomicExch(g.status, 1);
+    if (warp == 17) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+// tensor map of rows of x [rows][K]: boxes of 64 columns x `tokens` rows, 128-byte swizzle, zeros behind the edges
+int w4_x_map(CUtensorMap* map, const W4& a, int tokens, bool bf16)
+{
+    const EncodeTiledFn fn = encode_tiled();
+    if (!fn) return fail(NQ_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+    const cuuint64_t dims[2] = {(cuuint64_t)a.K, (cuuint64_t)a.rows}, strides[1] = {(cuuint64_t)a.x_stride * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)tokens}, estr[2] = {1, 1};
+    const CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(a.x), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(NQ_ERR_CUDA, "nq_w4_matmul: cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return NQ_OK;
+}
+
+template <class X, class SC, int GROUPS, int TOKENS>
+int wg_launch(Wg g, int device, cudaStream_t st)
+{
+    using Plan = WgPlan<GROUPS, TOKENS>;
+    W4& a = g.w;
+    CUtensorMap map;
+    if (int e = w4_x_map(&map, a, TOKENS, std::is_same<X, __nv_bfloat16>::value)) return e;
+    auto* kernel = w4_gemm_kernel<X, SC, GROUPS, TOKENS>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Plan::kSmem) != cudaSuccess) return fail(NQ_ERR_CUDA, "nq_w4_matmul: shared memory");
+    a.blocks = (a.S - 1) / 8 + 1;
+    const long long most = (long long)a.blocks * (a.start ? a.rows / TOKENS + (a.E < a.rows ? a.E : a.rows) : (a.rows - 1) / TOKENS + 1);
+    NQ_REQUIRE(most <= 0x7fffffff / a.C, "nq_w4_matmul: %d rows are too many", a.rows);
+    // columns are split while that leaves a cluster for every item
+    g.log_ck = 0;
+    while (!a.start && g.log_ck < 3 && a.C >> (g.log_ck + 1) >= 2 && most << (g.log_ck + 1) <= a.sms) ++g.log_ck;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1 << g.log_ck; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = 2;
+    const long long clusters = g.log_ck ? most : most < a.sms ? most : a.sms;
+    cfg.gridDim = dim3((unsigned)(clusters << g.log_ck)); cfg.blockDim = dim3(kWgThreads); cfg.dynamicSmemBytes = Plan::kSmem; cfg.stream = st;
+    cudaLaunchKernelEx(&cfg, kernel, map, g);
+    return check_launch("nq_w4_matmul");
+}
+template <class X, class SC, int GROUPS>
+int wg_tokens(const Wg& g, int device, cudaStream_t st)
+{
+    if (g.w.rows <= 32) return wg_launch<X, SC, GROUPS, 32>(g, device, st);
+    if (g.w.rows <= 64) return wg_launch<X, SC, GROUPS, 64>(g, device, st);
+    return wg_launch<X, SC, GROUPS, 128>(g, device, st);
+}
+template <class X, class SC>
+int wg_groups(const Wg& g, int group, int device, cudaStream_t st)
+{
+    return group == 128 ? wg_tokens<X, SC, 1>(g, device, st) : group == 64 ? wg_tokens<X, SC, 2>(g, device, st) : wg_tokens<X, SC, 4>(g, device, st);
+}
+
+int w4_gemm(const W4& a, int* status, int type, int sc_type, int group, int device, cudaStream_t st)
+{
+    const Wg g{a, status, 0};
+    if (type == NQ_F16) return sc_type == NQ_F16 ? wg_groups<__half, __half>(g, group, device, st) : wg_groups<__half, __nv_bfloat16>(g, group, device, st);
+    return sc_type == NQ_F16 ? wg_groups<__nv_bfloat16, __half>(g, group, device, st) : wg_groups<__nv_bfloat16, __nv_bfloat16>(g, group, device, st);
+}
+
+}  // namespace nq

@@ -57,10 +57,15 @@ class W4:
         s._zp = None if zeros is None else torch.empty(n.value * per, dtype=torch.uint8, device=q.device)
         q, scales, zeros = q.contiguous(), scales.contiguous(), None if zeros is None else zeros.contiguous()
         # addresses of the planes, for the calls
-        s._planes = s._qw.data_ptr(), s._sc.data_ptr(), _TYPE[scales.dtype], None if zeros is None else s._zp.data_ptr()
+        s._status = torch.zeros(1, dtype=torch.int32, device=q.device)
+        s._planes = s._qw.data_ptr(), s._sc.data_ptr(), _TYPE[scales.dtype], None if zeros is None else s._zp.data_ptr(), s._status.data_ptr()
         s._index = q.get_device()
         launch("W4", lib().nq_w4_layout, q, q.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), s.E, s.N, s.K, s.group,
                s._planes[0], s._planes[1], s._planes[3])
+
+    def status(s):
+        """0, or 1 if a device-side wait of a call has run out (its results are then invalid).  Synchronises."""
+        return int(s._status.item())
 
     def nbytes(s):
         """bytes of the planes on the device"""
@@ -89,7 +94,7 @@ class W4:
         if cols != 1 or rows < K or rows % 8 or x.data_ptr() % 16:
             x, rows = x.clone(memory_format=torch.contiguous_format), K      # rows that the kernel reads start on 16 bytes
         out = torch.empty((T, s.N), dtype=dtype, device=s.device)
-        qw, sc, sc_type, zp = s._planes
+        qw, sc, sc_type, zp, status = s._planes
         launch("W4", lib().nq_w4_matmul, x, x.data_ptr(), _TYPE[own], rows, qw, sc, sc_type, zp, None if start is None else start.data_ptr(), T, s.E, s.N, K,
-               s.group, out.data_ptr(), _TYPE[dtype], s.N)
+               s.group, out.data_ptr(), _TYPE[dtype], s.N, status)
         return out

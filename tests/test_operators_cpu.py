@@ -25,7 +25,7 @@ DISPATCH_BWD = dict(dxs=P, type=NQ_F16, pos=P, live=P, T=4, topk=2, H=64, dx=P, 
 COMBINE = dict(y=P, type=NQ_F16, rw=P, rw_type=NQ_F32, pos=P, live=P, T=4, topk=2, H=64, out=P, out_type=NQ_F32, stream=None)
 COMBINE_BWD = dict(dout=P, out_type=NQ_F16, y=P, type=NQ_F16, rw=P, rw_type=NQ_F32, pos=P, live=P, T=4, topk=2, H=64, dy=P, drw=P, stream=None)
 LAYOUT = dict(q=P, scales=P, zeros=P, E=2, N=64, K=256, group=64, qw=P, sc=P, zp=P, stream=None)
-MATMUL = dict(x=P, type=NQ_F16, x_stride=256, qw=P, sc=P, sc_type=NQ_F16, zp=P, start=P, rows=4, E=2, N=64, K=256, group=64, out=P, out_type=NQ_F32, out_stride=64, stream=None)
+MATMUL = dict(x=P, type=NQ_F16, x_stride=256, qw=P, sc=P, sc_type=NQ_F16, zp=P, start=P, rows=4, E=2, N=64, K=256, group=64, out=P, out_type=NQ_F32, out_stride=64, status=P, stream=None)
 
 
 @pytest.mark.skipif(torch.cuda.is_available(), reason="the arguments are not device addresses")
@@ -41,7 +41,7 @@ MATMUL = dict(x=P, type=NQ_F16, x_stride=256, qw=P, sc=P, sc_type=NQ_F16, zp=P, 
     ("nq_combine_bwd", COMBINE_BWD, [dict(type=7), dict(rw_type=9), dict(out_type=NQ_BF16), dict(T=-1), dict(H=0), dict(dout=None), dict(y=None), dict(rw=None), dict(pos=None)]),
     ("nq_w4_layout", LAYOUT, [dict(group=16), dict(group=256), dict(K=96, group=64), dict(K=0), dict(N=0), dict(E=0), dict(q=None), dict(zp=None), dict(zeros=None), dict(qw=P + 8)]),
     ("nq_w4_matmul", MATMUL, [dict(type=NQ_F32), dict(sc_type=NQ_F32), dict(out_type=NQ_BF16), dict(group=48), dict(K=320, group=128), dict(rows=-1), dict(start=None), dict(x_stride=255),
-                              dict(x_stride=260), dict(out_stride=63), dict(x=P + 8), dict(x=None), dict(qw=None), dict(sc=None), dict(out=None), dict(E=0), dict(E=70000)]),
+                              dict(x_stride=260), dict(out_stride=63), dict(x=P + 8), dict(x=None), dict(qw=None), dict(sc=None), dict(out=None), dict(status=None), dict(E=0), dict(E=1025)]),
 ] for o in overs], ids=lambda v: v if isinstance(v, str) else ",".join(f"{a}={b}" for a, b in v.items()) if len(v) < 4 else "")
 def test_c_entry_points_refuse(name, base, over):
     assert _with(getattr(capi.lib(), name), base, **over) == ARG
