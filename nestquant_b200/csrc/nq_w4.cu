@@ -290,7 +290,7 @@ int w4_clusters(K* kernel, int ck, int sms, int device, cudaLaunchConfig_t& cfg)
 // How a matrix is cut: CTAs of a cluster and warps of a CTA that share a strip, both powers of two.  The device takes ceil(blocks / clusters) rounds; a round
 // costs a warp its units and what comes per item (measured: sums and barriers as much as a unit and a half, over a cluster three).
 // calls for the other kernel
-bool w4_many_rows(int rows, int E, const int* start) { return rows > 32 && (!start || rows / E > 32); }
+bool w4_many_rows(int rows, int E, const int* start) { return (start ? rows / E : rows) > 16; }
 
 template <class X, class SC, int GROUPS, int TILES>
 bool w4_cut(W4& a, int rows, int device, cudaLaunchConfig_t& cfg, long long& clusters)
@@ -351,10 +351,10 @@ int w4_launch(W4 a, int device, cudaStream_t st)
 template <class X, class SC, int GROUPS>
 int w4_tiles(const W4& a, int device, cudaStream_t st)
 {
-    // as many tiles of eight rows as the call has, up to four; fewer where shared memory does not hold that many rows
-    const int pitch = w4_pitch(a.C, a.C < 8 ? a.C : 8);
-    if (a.rows <= 8 || 16 * pitch > W4Plan<GROUPS, 2>::kRoom) return w4_launch<X, SC, GROUPS, 1>(a, device, st);
-    if (a.rows <= 16 || 32 * pitch > W4Plan<GROUPS, 4>::kRoom) return w4_launch<X, SC, GROUPS, 2>(a, device, st);
+    // as many tiles of eight rows as the call has, or an expert on average; fewer where shared memory does not hold that many rows
+    const int pitch = w4_pitch(a.C, a.C < 8 ? a.C : 8), rows = a.start ? a.rows / a.E : a.rows;
+    if (rows <= 8 || 16 * pitch > W4Plan<GROUPS, 2>::kRoom) return w4_launch<X, SC, GROUPS, 1>(a, device, st);
+    if (rows <= 16 || 32 * pitch > W4Plan<GROUPS, 4>::kRoom) return w4_launch<X, SC, GROUPS, 2>(a, device, st);
     return w4_launch<X, SC, GROUPS, 4>(a, device, st);
 }
 template <class X, class SC>

@@ -139,7 +139,8 @@ struct W4Unit {
 };
 // A warp's units on their way through shared memory, DEPTH of them asked for ahead.  A lane copies the weights that it reads itself; the first lane of
 // four copies the scales and zero points of their two rows.
-template <int GROUPS, int DEPTH>
+// STEP: every unit of the strip, or every other one.
+template <int GROUPS, int DEPTH, int STEP = 1>
 struct W4Stream {
     static constexpr int kDepth = DEPTH, kScales = 1024, kZeros = kScales + 32 * GROUPS, kStage = kZeros + 16 * GROUPS, kBytes = kDepth * kStage;
     const char *w, *sc, *zp;             // of the next unit to ask for
@@ -170,8 +171,8 @@ struct W4Stream {
                 copy_async<4 * GROUPS>(place + at_sc, sc);
                 if (zeros) copy_async<GROUPS == 4 ? 8 : 4>(place + (at_zp & ~3), zp);
             }
-            w += 1024; sc += 32 * GROUPS;
-            if (zeros) zp += 16 * GROUPS;
+            w += STEP * 1024; sc += STEP * 32 * GROUPS;
+            if (zeros) zp += STEP * 16 * GROUPS;
         }
         copies_end();
         place = place == last ? last - (kDepth - 1) * kStage : place + kStage;

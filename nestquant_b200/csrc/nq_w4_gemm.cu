@@ -1,20 +1,18 @@
 // Products with 4-bit weights (nq_w4.cuh) for calls of many rows: on the fifth-generation tensor cores, 128 rows of the matrix times TOKENS rows of x per item.
 //
-//   warps 0..7    sums: each has 32 rows of the matrix (its quarter of tensor memory) and half of the tokens; adds every group's sums, times the
-//                 group's scale, to its registers, and writes the item's results
-//   warps 8..15   weights: each streams one strip of 16 rows (W4Stream), turns a unit into exact halves q - z and stores them as the MMA's A operand
-//                 in tensor memory (16x256b stores take the fragments as they are)
-//   warp 16       TMA: the tokens' tiles [TOKENS x 64], two per chunk of 128 columns
-//   warp 17       one lane issues tcgen05.mma, 128 x TOKENS x 16 a step, into one of two accumulators per group of columns: an accumulator holds one
-//                 group's sum only, so that the scale is applied in 32 bits and nothing is rounded before the result
+//   sums       (8 warps) a warp has 32 rows of the matrix (its quarter of tensor memory) and half of the tokens; adds every
+//              group's sums, times the group's scale, to its registers, and writes the item's results
+//   weights    (8 warps for 128 tokens, else 16) a warp streams one strip of 16 rows, or every other chunk of it (W4Stream), turns a unit into exact
+//              halves q - z and stores them as the MMA's A operand in tensor memory (16x256b stores take the fragments as they are)
+//   TMA        (one warp) the tokens' tiles [TOKENS x 64], two per chunk of 128 columns
+//   MMAs       (one warp) an elected lane issues tcgen05.mma, 128 x TOKENS x 16 a step, into one of two accumulators per group of columns: an accumulator
+//              holds one group's sum only, so that the scale is applied in 32 bits and nothing is rounded before the result
 // Columns of an item may be split over a cluster; each CTA then adds up a share of the tokens, the others' sums come through distributed shared memory.
 // Every mbarrier wait is bounded (nq_tc.cuh): on time-out the CTA raises status[0], waits for its loads and MMAs in flight and ends.
 #include "nq_tc.cuh"
 #include "nq_w4.cuh"
 
 namespace nq {
-
-constexpr int kWgSumWarps = 8, kWgDecodeWarps = 8, kWgThreads = 32 * (kWgSumWarps + kWgDecodeWarps + 2);
 
 struct WgShared {
     uint64_t full_a[6], full_b[6], empty[6], sum_full[2], sum_empty[2], done;
@@ -24,10 +22,15 @@ struct WgShared {
 };
 template <int GROUPS, int TOKENS>
 struct WgPlan {
-    using Stream = W4Stream<GROUPS, 4>;
+    static constexpr int kSumWarps = 8, kDecodeWarps = TOKENS == 128 ? 8 : 16, kHalves = kDecodeWarps / 8;      // (kHalves warps to a strip)
+    static constexpr int kTma = kSumWarps + kDecodeWarps, kMma = kTma + 1;                                      // the other two warps
+    static constexpr bool kSplit = TOKENS == 128;                         // registers go by warpgroup: 144 for sums, 72 for weights, 48 for the rest, of 5 x 96
+    static constexpr int kThreads = kSplit ? 640 : 32 * 26;
+    static constexpr int kColumns = TOKENS / 2;                           // tokens of a sum warp
+    using Stream = W4Stream<GROUPS, 4, kHalves>;
     static constexpr int kStages = TOKENS == 128 ? 4 : 6;                 // chunks ahead; a weight tile is 64 columns of tensor memory
     static constexpr int kBox = TOKENS * 128;                             // a token tile of 64 columns
-    static constexpr int kTiles = kStages * 2 * kBox, kPlanes = kWgDecodeWarps * Stream::kBytes, kSums = TOKENS * 512;
+    static constexpr int kTiles = kStages * 2 * kBox, kPlanes = kDecodeWarps * Stream::kBytes, kSums = TOKENS * 512;
     // tiles, and after them, or in their place once they are through, the sums of a split item; planes
     static constexpr int kRest = kTiles > kSums ? kTiles : kSums, kSmem = kRest + kPlanes + (int)sizeof(WgShared);
     static_assert(kSmem <= 232448, "shared memory of a CTA");
@@ -43,14 +46,25 @@ __device__ __forceinline__ void tma_two_boxes(uint32_t dst, uint32_t box, const 
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                  ::"r"(dst + box), "l"(map), "r"(x + 64), "r"(y), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void mma_step(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add)
+// The MMAs of a group of STEPS steps of 16 columns and the commit to `full`, by one elected lane (one election, few instructions: this warp shares its scheduler
+// with busy ones).  Weights in tensor memory, 8 columns a step; tokens in shared memory, two tiles of 64 columns, BOX bytes apart (the descriptor counts in 16
+// bytes).  The first MMA overwrites the accumulator.
+#define NQ_WG_STEP(A, B, P) \
+    "add.u32 ta, %1, " A ";\n\tadd.u32 tb, %2, " B ";\n\tmov.b64 db, {tb, %3};\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ta], db, %4, " P ";\n\t"
+#define NQ_WG_GROUP(STEPS_TEXT)                                                                                                                       \
+    asm volatile("{\n\t.reg .pred p, q, e;\n\t.reg .b64 db;\n\t.reg .b32 ta, tb;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 p, %4, %4;\n\tsetp.eq.u32 q, %4, %4;\n\t"  \
+                 STEPS_TEXT "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%5];\n\t}"                                     \
+                 ::"r"(d), "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(full), "n"(BOX >> 4) : "memory")
+template <int STEPS, int BOX>
+__device__ __forceinline__ void mma_group(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t full)
 {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
-}
-__device__ __forceinline__ void commit(uint64_t* bar)
-{
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(saddr(bar)) : "memory");
+    if constexpr (STEPS == 8)
+        NQ_WG_GROUP(NQ_WG_STEP("0", "0", "p") NQ_WG_STEP("8", "2", "q") NQ_WG_STEP("16", "4", "q") NQ_WG_STEP("24", "6", "q")
+                    NQ_WG_STEP("32", "%6", "q") NQ_WG_STEP("40", "%6+2", "q") NQ_WG_STEP("48", "%6+4", "q") NQ_WG_STEP("56", "%6+6", "q"));
+    else if constexpr (STEPS == 4)
+        NQ_WG_GROUP(NQ_WG_STEP("0", "0", "p") NQ_WG_STEP("8", "2", "q") NQ_WG_STEP("16", "4", "q") NQ_WG_STEP("24", "6", "q"));
+    else
+        NQ_WG_GROUP(NQ_WG_STEP("0", "0", "p") NQ_WG_STEP("8", "2", "q"));
 }
 __device__ __forceinline__ void tmem_ld16_async(uint32_t taddr, uint32_t (&v)[16])
 {
@@ -67,6 +81,59 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t (&v)[16])
                    "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]) :: "memory");
 }
 
+// two 32-bit floats in a register pair
+__device__ __forceinline__ uint64_t two_floats(float v) { return (uint64_t)__float_as_uint(v) << 32 | __float_as_uint(v); }
+__device__ __forceinline__ float one_of(uint64_t v, int i) { return __uint_as_float((uint32_t)(i ? v >> 32 : v)); }
+// sum += s * (x, y)
+__device__ __forceinline__ void fma_two(uint64_t& sum, uint64_t s, uint32_t x, uint32_t y)
+{
+    asm("{\n\t.reg .b64 v;\n\tmov.b64 v, {%2, %3};\n\tfma.rn.f32x2 %0, %1, v, %0;\n\t}" : "+l"(sum) : "l"(s), "r"(x), "r"(y));
+}
+
+// (mbar_wait_warp with its slow part in line: a call would take the registers that the sums are in)
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, PfWaits* waits)
+{
+    unsigned long long t0 = 0, t;
+    while (!__all_sync(0xffffffffu, mbar_poll(bar, parity)))
+    {
+        if (__any_sync(0xffffffffu, waits->aborted)) return false;
+        asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+        if (t0 == 0) t0 = t;
+        else if (__any_sync(0xffffffffu, t - t0 > waits->limit_ns)) { waits->aborted = 1; return false; }
+    }
+    return true;
+}
+// (likewise mbar_wait_own)
+__device__ __forceinline__ void wait_own(uint32_t bar, uint32_t parity)
+{
+    unsigned long long t0 = 0, t = 0;
+    while (!__all_sync(0xffffffffu, mbar_poll(bar, parity)))
+    {
+        asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+        if (t0 == 0) t0 = t;
+        else if (__any_sync(0xffffffffu, t - t0 > (unsigned long long)kPfWaitNs)) return;
+    }
+}
+// a column of results, the first `there` of them
+template <class O, int N>
+__device__ __forceinline__ void store_column(O* to, long long stride, const uint64_t (&sum)[N], int there)
+{
+#pragma unroll
+    for (int t = 0; t < 2 * N; ++t)
+    {
+        if (t < there) *to = from_float<O>(one_of(sum[t / 2], t & 1));
+        to += stride;
+    }
+}
+// all threads of the cluster, warp by warp
+__device__ __forceinline__ void cluster_meet()
+{
+    tc_fence_before();
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+}
+
 struct Wg {
     W4 w;
     int* status;
@@ -77,11 +144,11 @@ struct Wg {
 template <int N>
 struct Ring {
     uint32_t s = 0, parity = 0;
-    __device__ __forceinline__ void next() { if (++s == N) { s = 0; parity ^= 1u; } }
+    __device__ __forceinline__ void next(uint32_t by = 1) { if ((s += by) >= N) { s -= N; parity ^= 1u; } }
 };
 
 template <class X, class SC, int GROUPS, int TOKENS>
-__global__ void __launch_bounds__(kWgThreads, 1) w4_gemm_kernel(const __grid_constant__ CUtensorMap map, Wg g)
+__global__ void __launch_bounds__((WgPlan<GROUPS, TOKENS>::kThreads), 1) w4_gemm_kernel(const __grid_constant__ CUtensorMap map, Wg g)
 {
     using Plan = WgPlan<GROUPS, TOKENS>;
     using Stream = typename Plan::Stream;
@@ -101,13 +168,13 @@ __global__ void __launch_bounds__(kWgThreads, 1) w4_gemm_kernel(const __grid_con
     const bool zeros = a.zp != nullptr;
     if (threadIdx.x == 0)
     {
-        for (int s = 0; s < kStages; ++s) { mbar_init(&sh.full_a[s], kWgDecodeWarps); mbar_init(&sh.full_b[s], 1); mbar_init(&sh.empty[s], 1); }
-        for (int s = 0; s < 2; ++s) { mbar_init(&sh.sum_full[s], 1); mbar_init(&sh.sum_empty[s], kWgSumWarps); }
+        for (int s = 0; s < kStages; ++s) { mbar_init(&sh.full_a[s], 8); mbar_init(&sh.full_b[s], 1); mbar_init(&sh.empty[s], 1); }
+        for (int s = 0; s < 2; ++s) { mbar_init(&sh.sum_full[s], 1); mbar_init(&sh.sum_empty[s], Plan::kSumWarps); }
         mbar_init(&sh.done, 1);
         sh.waits.aborted = 0; sh.waits.limit_ns = (unsigned long long)kPfWaitNs;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 17)
+    if (warp == Plan::kMma)
     {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(&sh.tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -137,97 +204,112 @@ __global__ void __launch_bounds__(kWgThreads, 1) w4_gemm_kernel(const __grid_con
         base = sh.row[c.e] + (c.pass - sh.first[c.e]) * TOKENS;
         return min(max(sh.row[c.e + 1], sh.row[c.e]) - base, TOKENS);
     };
-    float sum[TOKENS / 2];                                // of warps 0 to 7
-    int last_base = 0, last_rows = 0, last_block = 0;
-    if (warp < kWgSumWarps)
+    constexpr int kColumns = Plan::kColumns;
+    if (warp < Plan::kSumWarps)
     {
+        if (Plan::kSplit) asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
         // ---- sums
-        const int quarter = warp & 3, half = warp >> 2;
-        const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + half * (TOKENS / 2);
+        const int quarter = warp & 3, t0 = (warp >> 2) * kColumns, r = quarter * 32 + lane;
+        const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + t0;
+        uint64_t sum[kColumns / 2];                       // two tokens in each
         Ring<2> acc;
         bool ok = true;
         for (int i = i0; i < i1 && ok; ++i, now.next(blocks, sh.first, a.E, passes))
         {
             int base;
-            const int rows = rows_of(now, base), r = quarter * 32 + lane;
+            const int rows = rows_of(now, base);
             const size_t unit = ((size_t)now.e * a.S + min(now.block * 8 + r / 16, a.S - 1)) * a.C;
-            const uint16_t* sc = a.sc + unit * 16 * GROUPS + (r & 7) * 2 * GROUPS + (r >> 3 & 1);
+            const uint16_t* sc = a.sc + (unit + c0) * 16 * GROUPS + (r & 7) * 2 * GROUPS + (r >> 3 & 1);
             // scales two chunks ahead
             uint16_t next[2][GROUPS];
 #pragma unroll
             for (int d = 0; d < 2; ++d)
 #pragma unroll
-                for (int j = 0; j < GROUPS; ++j) next[d][j] = c0 + d < c1 ? sc[(size_t)(c0 + d) * 16 * GROUPS + 2 * j] : 0;
+                for (int j = 0; j < GROUPS; ++j) next[d][j] = c0 + d < c1 ? sc[d * 16 * GROUPS + 2 * j] : 0;
 #pragma unroll
-            for (int j = 0; j < TOKENS / 2; ++j) sum[j] = 0.f;
+            for (int j = 0; j < kColumns / 2; ++j) sum[j] = 0;
             for (int c = c0; c < c1 && ok; ++c)
             {
                 uint16_t scale[GROUPS];
+                sc += 16 * GROUPS;
 #pragma unroll
                 for (int j = 0; j < GROUPS; ++j)
                 {
                     scale[j] = next[0][j];
                     next[0][j] = next[1][j];
-                    next[1][j] = c + 2 < c1 ? sc[(size_t)(c + 2) * 16 * GROUPS + 2 * j] : 0;
+                    next[1][j] = c + 2 < c1 ? sc[16 * GROUPS + 2 * j] : 0;
                 }
 #pragma unroll
                 for (int j = 0; j < GROUPS; ++j)
                 {
-                    ok = ok && mbar_wait_warp(saddr(&sh.sum_full[acc.s]), acc.parity, &sh.waits);
+                    ok = ok && wait_bar(saddr(&sh.sum_full[acc.s]), acc.parity, &sh.waits);
                     if (!ok) break;
                     tc_fence_after();
-                    const float s = scales_of<SC>(scale[j]).x;
+                    const uint64_t s = two_floats(scales_of<SC>(scale[j]).x);
+                    constexpr int kAtOnce = kColumns < 32 ? kColumns : 32;
 #pragma unroll
-                    for (int t0 = 0; t0 < TOKENS / 2; t0 += 32)
+                    for (int k0 = 0; k0 < kColumns; k0 += kAtOnce)
                     {
-                        uint32_t v[16], w[16];
-                        constexpr bool kTwo = TOKENS >= 64;
-                        tmem_ld16_async(from + acc.s * TOKENS + t0, v);
-                        if (kTwo) tmem_ld16_async(from + acc.s * TOKENS + t0 + 16, w);
-                        tmem_wait_ld(v);
-                        if (kTwo) tmem_wait_ld(w);
-                        if (t0 + 32 >= TOKENS / 2)
+                        uint32_t v[kAtOnce / 16][16];
+#pragma unroll
+                        for (int h = 0; h < kAtOnce / 16; ++h) tmem_ld16_async(from + acc.s * TOKENS + k0 + 16 * h, v[h]);
+#pragma unroll
+                        for (int h = 0; h < kAtOnce / 16; ++h) tmem_wait_ld(v[h]);
+                        if (k0 + kAtOnce == kColumns)
                         {
                             tc_fence_before();
                             __syncwarp();
                             if (lane == 0) mbar_arrive(&sh.sum_empty[acc.s]);
                         }
 #pragma unroll
-                        for (int k = 0; k < 16; ++k) sum[t0 + k] += s * __uint_as_float(v[k]);
-                        if (kTwo)
-#pragma unroll
-                            for (int k = 0; k < 16; ++k) sum[(t0 + 16 + k) % (TOKENS / 2)] += s * __uint_as_float(w[k]);
+                        for (int k = 0; k < kAtOnce / 2; ++k) fma_two(sum[k0 / 2 + k], s, v[k / 8][2 * k % 16], v[k / 8][2 * k % 16 + 1]);
                     }
                     acc.next();
                 }
             }
-            last_base = base; last_rows = rows; last_block = now.block;
             if (ck == 1 && ok)
             {
-                const int n = now.block * 128 + r;
-                if (n < a.N)
+                const int n = now.block * 128 + r, there = n < a.N ? rows - t0 : 0;
+                const size_t first = (size_t)(base + t0) * a.out_stride + n;
+                if (a.out_type == NQ_F32) store_column<float>((float*)a.out + first, a.out_stride, sum, there);
+                else store_column<X>((X*)a.out + first, a.out_stride, sum, there);
+            }
+        }
+        if (ck > 1)
+        {
+            // one item: when every CTA of the cluster is through with its tiles, their place takes the sums: [rank][token of the CTA's share][row]
+            cluster_meet();
+            const int log_share = 31 - __clz(TOKENS >> g.log_ck), share = 1 << log_share;
 #pragma unroll
-                    for (int t = 0; t < TOKENS / 2; ++t)
-                        if (half * (TOKENS / 2) + t < rows) store_as(a.out, a.out_type, (size_t)(base + half * (TOKENS / 2) + t) * a.out_stride + n, sum[t]);
+            for (int t = 0; t < kColumns; ++t)
+            {
+                const int token = t0 + t;
+                const uint32_t at = cluster_address(saddr(wg_smem) + ((((rank << log_share) + (token & (share - 1))) << 7) + r) * 4, token >> log_share);
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(one_of(sum[t / 2], t & 1)) : "memory");
             }
         }
     }
-    else if (warp < kWgSumWarps + kWgDecodeWarps)
+    else if (warp < Plan::kTma)
     {
-        // ---- weights.  A warp reaches the quarter of tensor memory that its number has: strips 2 (warp % 4) and the one behind it
-        const int strip = 2 * (warp & 3) + (warp >> 2 & 1);
-        Stream planes((const char*)s_planes + (warp - kWgSumWarps) * Stream::kBytes, lane);
+        if (Plan::kSplit) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        // ---- weights.  A warp reaches the quarter of tensor memory that its number has: strips 2 (warp % 4) and the one behind it.  Chunks are counted over all
+        // items; of two warps to a strip one has the even ones, the other the odd ones.
+        constexpr int kHalves = Plan::kHalves;
+        const int who = warp - Plan::kSumWarps, strip = 2 * (warp & 3) + (who >> 2 & 1), half = who >> 3, chunks = c1 - c0;
+        Stream planes((const char*)s_planes + who * Stream::kBytes, lane);
         W4Cursor ahead = now;
-        int to_ask = i1 - i0, left = 0;
+        int to_ask = i1 - i0, left = 0, parity = half;    // (parity: of the next item's first chunk that is this warp's)
         bool there = true;
         auto ask = [&] {
-            if (--left < 0)
+            while (--left < 0)
             {
                 if (to_ask-- > 0)
                 {
-                    planes.seek(a, ((size_t)ahead.e * a.S + min(ahead.block * 8 + strip, a.S - 1)) * a.C + c0, lane);
+                    const int skip = kHalves == 2 ? parity : 0;
+                    planes.seek(a, ((size_t)ahead.e * a.S + min(ahead.block * 8 + strip, a.S - 1)) * a.C + c0 + skip, lane);
                     ahead.next(blocks, sh.first, a.E, passes);
-                    left = c1 - c0 - 1;
+                    left = kHalves == 2 ? (chunks - skip + 1) >> 1 : chunks;
+                    parity ^= chunks & 1;
                 }
                 else { there = false; left = 0x7fffffff; }
             }
@@ -237,13 +319,13 @@ __global__ void __launch_bounds__(kWgThreads, 1) w4_gemm_kernel(const __grid_con
         for (int d = 0; d < Stream::kDepth; ++d) ask();
         const uint32_t to = tmem + ((uint32_t)(strip * 16) << 16) + 2 * TOKENS;
         Ring<kStages> stage;
-        for (int u = (i1 - i0) * (c1 - c0); u > 0; --u)
+        stage.s = half;
+        uint32_t stored = 0;                              // barrier of the unit whose stores are on their way
+        for (int u = (i1 - i0) * chunks - half; u > 0; u -= kHalves)
         {
             W4Unit<GROUPS> unit;
             planes.oldest(unit, zeros);
             const uint32_t words[8] = {unit.w[0].x, unit.w[0].y, unit.w[0].z, unit.w[0].w, unit.w[1].x, unit.w[1].y, unit.w[1].z, unit.w[1].w};
-            if (!mbar_wait_warp(saddr(&sh.empty[stage.s]), stage.parity ^ 1u, &sh.waits)) break;
-            tc_fence_after();
 #pragma unroll
             for (int h = 0; h < 2; ++h)
             {
@@ -258,18 +340,40 @@ __global__ void __launch_bounds__(kWgThreads, 1) w4_gemm_kernel(const __grid_con
                     Operand<X>::weights(words[4 * h + j], lo, hi, f);
                     r[4 * j] = f[0]; r[4 * j + 1] = f[2]; r[4 * j + 2] = f[1]; r[4 * j + 3] = f[3];
                 }
+                if (h == 0)
+                {
+                    // the unit before this one has been stored by now
+                    if (stored)
+                    {
+                        tmem_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive32(stored);
+                    }
+                    stored = 0;
+                    if (!wait_bar(saddr(&sh.empty[stage.s]), stage.parity ^ 1u, &sh.waits)) { u = 0; break; }
+                    tc_fence_after();
+                }
                 tmem_st_16x256b_x4(to + stage.s * 64 + h * 32, r);
             }
+            if (u == 0) break;
+            stored = saddr(&sh.full_a[stage.s]);
             ask();
+            stage.next(kHalves);
+        }
+        if (stored)
+        {
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.full_a[stage.s]);
-            stage.next();
+            if (lane == 0) mbar_arrive32(stored);
         }
         copies_done<0>();
     }
-    else if (warp == 16)
+    else
+    {
+    if (Plan::kSplit) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    if (warp == Plan::kTma)
     {
         // ---- token tiles
         if (!a.start) grid_dependency_wait();
@@ -283,7 +387,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) w4_gemm_kernel(const __grid_con
             rows_of(now, base);
             for (int c = c0; c < c1; ++c)
             {
-                ok = mbar_wait_warp(saddr(&sh.empty[stage.s]), stage.parity ^ 1u, &sh.waits);
+                ok = wait_bar(saddr(&sh.empty[stage.s]), stage.parity ^ 1u, &sh.waits);
                 if (!ok) break;
                 if (lane == 0) tma_two_boxes(tiles + stage.s * 2 * Plan::kBox, Plan::kBox, &map, c * 128, base, saddr(&sh.full_b[stage.s]));
                 __syncwarp();
@@ -291,70 +395,49 @@ __global__ void __launch_bounds__(kWgThreads, 1) w4_gemm_kernel(const __grid_con
                 stage.next();
             }
         }
-        for (int s = 0; s < kStages; ++s) mbar_wait_own(saddr(&sh.full_b[s]), ((asked >> s) & 1u) ^ 1u);      // loads on their way
+        for (int s = 0; s < kStages; ++s) wait_own(saddr(&sh.full_b[s]), ((asked >> s) & 1u) ^ 1u);      // loads on their way
     }
-    else
+    else if (warp == Plan::kMma)
     {
         // ---- MMAs
         constexpr uint32_t kType = std::is_same<X, __half>::value ? 0u : 1u;
         constexpr uint32_t kDesc = (1u << 4) | (kType << 7) | (kType << 10) | ((uint32_t)(TOKENS >> 3) << 17) | (8u << 24);      // fp32 sums, both operands K-major, M 128
-        const uint64_t b0 = smem_desc(saddr(wg_smem), 16, 1024, 2);
+        const uint64_t desc = smem_desc(saddr(wg_smem), 16, 1024, 2);
+        const uint32_t b0 = (uint32_t)desc, b_hi = (uint32_t)(desc >> 32);
         Ring<kStages> stage;
         Ring<2> acc;
         bool ok = true;
         for (int u = (i1 - i0) * (c1 - c0); u > 0 && ok; --u)
         {
-            ok = mbar_wait_warp(saddr(&sh.full_a[stage.s]), stage.parity, &sh.waits) && mbar_wait_warp(saddr(&sh.full_b[stage.s]), stage.parity, &sh.waits);
-#pragma unroll
-            for (int j = 0; j < GROUPS; ++j)
-            {
-                ok = ok && mbar_wait_warp(saddr(&sh.sum_empty[acc.s]), acc.parity ^ 1u, &sh.waits);
-                if (!ok) break;
-                tc_fence_after();
-                if (lane == 0)
+            ok = wait_bar(saddr(&sh.full_a[stage.s]), stage.parity, &sh.waits) && wait_bar(saddr(&sh.full_b[stage.s]), stage.parity, &sh.waits);
+            const uint32_t w = tmem + 2 * TOKENS + stage.s * 64, b_lo = b0 + stage.s * (2 * Plan::kBox >> 4);
+            auto group = [&](auto j) {
+                constexpr int kSteps = 8 / GROUPS, kFirst = decltype(j)::value * kSteps;
+                if constexpr (kFirst < 8)
                 {
-                    const uint32_t d = tmem + acc.s * TOKENS, w = tmem + 2 * TOKENS + stage.s * 64;
-#pragma unroll
-                    for (int q = 0; q < 8 / GROUPS; ++q)
-                    {
-                        const int k = j * (8 / GROUPS) + q;       // step of the chunk
-                        mma_step(d, w + k * 8, b0 + ((stage.s * 2 * Plan::kBox + (k >> 2) * Plan::kBox + (k & 3) * 32) >> 4), kDesc, q != 0);
-                    }
-                    commit(&sh.sum_full[acc.s]);
-                    if (j == GROUPS - 1) commit(&sh.empty[stage.s]);
+                    ok = ok && wait_bar(saddr(&sh.sum_empty[acc.s]), acc.parity ^ 1u, &sh.waits);
+                    if (!ok) return;
+                    tc_fence_after();
+                    mma_group<kSteps, Plan::kBox>(tmem + acc.s * TOKENS, w + kFirst * 8, b_lo + (kFirst >> 2) * (Plan::kBox >> 4) + (kFirst & 3) * 2, b_hi, kDesc,
+                                                  saddr(&sh.sum_full[acc.s]));
+                    acc.next();
                 }
-                __syncwarp();
-                acc.next();
-            }
+            };
+            group(std::integral_constant<int, 0>()); group(std::integral_constant<int, 1>()); group(std::integral_constant<int, 2>()); group(std::integral_constant<int, 3>());
+            if (ok) tc_commit_elect(&sh.empty[stage.s]);
             stage.next();
         }
-        if (lane == 0) commit(&sh.done);
         __syncwarp();
-        mbar_wait_own(saddr(&sh.done), 0);
+        tc_commit_elect(&sh.done);
+        wait_own(saddr(&sh.done), 0);
     }
+    }
+    if (ck > 1 && warp >= Plan::kSumWarps) cluster_meet();
     launch_dependents();
     if (ck > 1)
     {
-        // one item: every CTA of the cluster is through with its tiles, whose place takes the sums: [rank][token of this CTA's share][row]
-        tc_fence_before();
-        __syncwarp();
-        cluster_arrive();
-        cluster_wait();
         const int share = TOKENS >> g.log_ck, log_share = 31 - __clz(share);
-        if (warp < kWgSumWarps && i0 < i1)
-        {
-            const int quarter = warp & 3, half = warp >> 2;
-#pragma unroll
-            for (int t = 0; t < TOKENS / 2; ++t)
-            {
-                const int token = half * (TOKENS / 2) + t;
-                const uint32_t at = cluster_address(saddr(wg_smem) + ((((rank << log_share) + (token & (share - 1))) << 7) + quarter * 32 + lane) * 4, token >> log_share);
-                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(sum[t]) : "memory");
-            }
-        }
-        __syncwarp();
-        cluster_arrive();
-        cluster_wait();
+        cluster_meet();
         if (i0 < i1)
         {
             // (what every thread needs of the item)
@@ -378,7 +461,7 @@ __global__ void __launch_bounds__(kWgThreads, 1) w4_gemm_kernel(const __grid_con
     tc_fence_before();
     __syncthreads();
     if (sh.waits.aborted && threadIdx.x == 0) atomicExch(g.status, 1);
-    if (warp == 17) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    if (warp == Plan::kMma) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 // tensor map of rows of x [rows][K]: boxes of 64 columns x `tokens` rows, 128-byte swizzle, zeros behind the edges
@@ -417,15 +500,16 @@ int wg_launch(Wg g, int device, cudaStream_t st)
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr; cfg.numAttrs = 2;
     const long long clusters = g.log_ck ? most : most < a.sms ? most : a.sms;
-    cfg.gridDim = dim3((unsigned)(clusters << g.log_ck)); cfg.blockDim = dim3(kWgThreads); cfg.dynamicSmemBytes = Plan::kSmem; cfg.stream = st;
+    cfg.gridDim = dim3((unsigned)(clusters << g.log_ck)); cfg.blockDim = dim3(Plan::kThreads); cfg.dynamicSmemBytes = Plan::kSmem; cfg.stream = st;
     cudaLaunchKernelEx(&cfg, kernel, map, g);
     return check_launch("nq_w4_matmul");
 }
 template <class X, class SC, int GROUPS>
 int wg_tokens(const Wg& g, int device, cudaStream_t st)
 {
-    if (g.w.rows <= 32) return wg_launch<X, SC, GROUPS, 32>(g, device, st);
-    if (g.w.rows <= 64) return wg_launch<X, SC, GROUPS, 64>(g, device, st);
+    const int rows = g.w.start ? g.w.rows / g.w.E * 3 / 2 : g.w.rows;      // (an expert of one and a half times the average should not take two passes)
+    if (rows <= 32) return wg_launch<X, SC, GROUPS, 32>(g, device, st);
+    if (rows <= 64) return wg_launch<X, SC, GROUPS, 64>(g, device, st);
     return wg_launch<X, SC, GROUPS, 128>(g, device, st);
 }
 template <class X, class SC>
