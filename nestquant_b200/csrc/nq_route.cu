@@ -13,7 +13,7 @@
 // exponential is computed.  |fp32 score - score| <= 1.8e-7 + 6e-8 |score|: expf has 2 ulp, which the slope s (1 - s) <= 1/4 makes
 // 6e-8; the sum and the quotient round once each, 6e-8 s; the bias adds 6e-8 |score|.  Two neighbours in the sorted list that are
 // further apart than 6e-7 + 3e-7 |score| are in the right order, and so are equal logits with equal biases; a row with any other
-// neighbours among its first topk + 1 is chosen again in 64 bits.
+// neighbours among its first topk + 1 is put in order again in 64 bits (one row of a thousand, with 256 experts).
 //
 // A warp per row; lane i holds the experts [i PER, (i + 1) PER), so that the lowest lane that has the largest key also has the lowest id.
 #include <cuda_bf16.h>
@@ -34,6 +34,9 @@ __device__ __forceinline__ unsigned float_key(float f)
 }
 __device__ __forceinline__ float key_float(unsigned k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 __device__ __forceinline__ bool eligible(float f) { return f > -INFINITY; }      // false for NaN
+// scores of about this size that are further apart than this are in the right order
+__device__ __forceinline__ float in_doubt_below(float score) { return 6e-7f + 3e-7f * fabsf(score); }
+__device__ __forceinline__ double exact_score(float l, float b) { return 1.0 / (1.0 + exp(-(double)l)) + (double)b; }
 __device__ __forceinline__ float sigmoid(float l) { return 1.f / (1.f + expf(-l)); }
 __device__ __forceinline__ float warp_sum(float v)
 {
@@ -70,26 +73,29 @@ __device__ __forceinline__ void load_run(const L* row, int e0, int E, bool vec, 
     }
 }
 
-// the row's choice again, in 64 bits: pick j goes to lane j.  The scores are recomputed for every pick: rows that come here are rare.
+// the row's choice again, in 64 bits: pick j goes to lane j
 template <class L, int PER>
 __device__ __noinline__ int choose_exactly(const L* row, const float* bias, int E, int topk)
 {
     const int lane = threadIdx.x & 31;
-    unsigned taken = 0;
+    double score[PER];
+    unsigned left = 0;                                     // experts of this lane that may be chosen
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+    {
+        const int e = lane * PER + i;
+        const float l = e < E ? to_float(row[e]) : -INFINITY, b = e < E ? bias[e] : -INFINITY;
+        score[i] = exact_score(l, b);
+        if (eligible(l) && eligible(b)) left |= 1u << i;
+    }
     int mine = -1;
     for (int j = 0; j < topk; ++j)
     {
         double best = 0.0;
         int at = -1;
+#pragma unroll
         for (int i = 0; i < PER; ++i)
-        {
-            const int e = lane * PER + i;
-            if (e >= E || (taken >> i & 1)) continue;
-            const float l = to_float(row[e]), b = bias[e];
-            if (!eligible(l) || !eligible(b)) continue;
-            const double s = 1.0 / (1.0 + exp(-(double)l)) + (double)b;
-            if (at < 0 || s > best) { best = s; at = i; }
-        }
+            if ((left >> i & 1) && (at < 0 || score[i] > best)) { best = score[i]; at = i; }
         // the largest, of the lowest lane that has it
         int from = lane;
         bool any = at >= 0;
@@ -101,11 +107,57 @@ __device__ __noinline__ int choose_exactly(const L* row, const float* bias, int 
             if (a && (!any || s > best || (s == best && w < from))) { best = s; from = w; any = true; }
         }
         if (!any) break;                                   // warp-uniform: every lane has the same answer
-        if (lane == from) taken |= 1u << at;
+        if (lane == from) left &= ~(1u << at);
         const int e = __shfl_sync(0xffffffffu, lane * PER + at, from);
         if (lane == j) mine = e;
     }
     return mine;
+}
+
+// the same among n candidates, one a lane
+template <class L>
+__device__ __noinline__ int rank_exactly(const L* row, const float* bias, uint2* found, int n, int topk)
+{
+    const int lane = threadIdx.x & 31, e = lane < n ? (int)found[lane].y : 0;
+    const double mine = lane < n ? exact_score(to_float(row[e]), bias[e]) : 0.0;
+    int before = 0;
+    for (int j = 0; j < n; ++j)
+    {
+        const double s = __shfl_sync(0xffffffffu, mine, j);
+        const int other = __shfl_sync(0xffffffffu, e, j);
+        before += s > mine || (s == mine && other < e);
+    }
+    __syncwarp();
+    if (lane < n) found[before].y = e;
+    __syncwarp();
+    return lane < topk && lane < n ? (int)found[lane].y : -1;
+}
+
+// The `picks` largest keys one by one, whatever they are; pick j to lane j, the last one (picks may be 33) also to next_key, next_e
+template <int PER>
+__device__ __noinline__ void choose_one_by_one(const unsigned (&keys)[PER], int picks, unsigned& my_key, int& my_e, unsigned& next_key, int& next_e)
+{
+    const int lane = threadIdx.x & 31;
+    unsigned key[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) key[i] = keys[i];
+    for (int j = 0; j < picks; ++j)
+    {
+        unsigned m = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) m = max(m, key[i]);
+        const unsigned top = __reduce_max_sync(0xffffffffu, m);
+        if (!top) break;
+        const int from = __ffs(__ballot_sync(0xffffffffu, m == top)) - 1;
+        int at = 0;
+#pragma unroll
+        for (int i = PER - 1; i >= 0; --i) at = key[i] == top ? i : at;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) key[i] = lane == from && i == at ? 0u : key[i];
+        const int e = __shfl_sync(0xffffffffu, lane * PER + at, from);
+        if (lane == j) { my_key = top; my_e = e; }
+        if (j == picks - 1) { next_key = top; next_e = e; }
+    }
 }
 
 struct Route {
@@ -161,28 +213,59 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(Route a)
         }
         key[i] = ok ? float_key(s) : 0u;
     }
-    // pick j to lane j; one more with a bias, to see how far the last one is from it
-    unsigned my_key = 0;
-    int my_e = -1;
+    // Pick j to lane j, and behind a biased choice the one that follows it.  No key below the picks-th largest of the lanes' largest keys is among the picks
+    // largest, so the few that are not go to the lanes, one each, and count how many are in front of them.  (Taking the largest away pick by pick cost
+    // 48 instructions a pick: 16,384 rows of 256 16.5 us.)
+    __shared__ uint2 s_found[kRouteWarps][2][34];          // {key, expert}: as found, in order
+    uint2 (&found)[2][34] = s_found[threadIdx.x >> 5];
+    unsigned my_key = 0, next_key = 0;
+    int my_e = -1, next_e = -1;
     const int picks = a.bias ? min(a.topk + 1, a.E) : a.topk;
-    unsigned next_key = 0;                                 // of pick topk, if it is looked at (topk may be 32: no lane is left for it)
-    int next_e = -1;
+    unsigned lead = 0, border = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) lead = max(lead, key[i]);
     for (int j = 0; j < picks; ++j)
     {
-        unsigned m = 0;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) m = max(m, key[i]);
-        const unsigned top = __reduce_max_sync(0xffffffffu, m);
+        const unsigned top = __reduce_max_sync(0xffffffffu, lead);
+        border = top;
         if (!top) break;
-        const int from = __ffs(__ballot_sync(0xffffffffu, m == top)) - 1;
-        int at = 0;
+        lead = lead == top ? 0u : lead;
+    }
+    border = max(border, 1u);
+    if (a.bias && border > 1u)                             // and what may be among them in 64 bits
+    {
+        const float f = key_float(border), lower = f - in_doubt_below(f);
+        border = lower > -INFINITY ? float_key(lower) : 1u;
+    }
+    int n = 0;
 #pragma unroll
-        for (int i = PER - 1; i >= 0; --i) at = key[i] == top ? i : at;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) key[i] = lane == from && i == at ? 0u : key[i];
-        const int e = __shfl_sync(0xffffffffu, lane * PER + at, from);
-        if (lane == j) { my_key = top; my_e = e; }
-        if (j == a.topk) { next_key = top; next_e = e; }
+    for (int i = 0; i < PER; ++i)
+    {
+        const bool in = key[i] >= border;
+        const unsigned m = __ballot_sync(0xffffffffu, in);
+        const int at = n + __popc(m & ((1u << lane) - 1u));
+        if (in && at < 32) found[0][at] = make_uint2(key[i], lane * PER + i);
+        n += __popc(m);
+    }
+    __syncwarp();
+    if (n <= 32 && picks <= 32)
+    {
+        const uint2 mine = lane < n ? found[0][lane] : make_uint2(0u, 0u);
+        int before = 0;
+        for (int j = 0; j < n; ++j)
+        {
+            const uint2 other = found[0][j];
+            before += other.x > mine.x || (other.x == mine.x && other.y < mine.y);
+        }
+        if (lane < n) found[1][before] = mine;
+        __syncwarp();
+        if (lane < a.topk && lane < n) { my_key = found[1][lane].x; my_e = (int)found[1][lane].y; }
+        if (a.topk < picks && a.topk < n) { next_key = found[1][a.topk].x; next_e = (int)found[1][a.topk].y; }
+    }
+    else
+    {
+        choose_one_by_one<PER>(key, picks, my_key, my_e, next_key, next_e);
+        if (picks == a.topk) next_e = -1;
     }
     if (a.bias)
     {
@@ -194,10 +277,11 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(Route a)
         if (lane < a.topk && my_e >= 0 && e1 >= 0)
         {
             const float s0 = key_float(my_key), s1 = key_float(k1);
-            const bool apart = s0 - s1 > 6e-7f + 3e-7f * fmaxf(fabsf(s0), fabsf(s1));
+            const bool apart = s0 - s1 > in_doubt_below(fmaxf(fabsf(s0), fabsf(s1)));
             if (!apart) doubt = !(to_float(row[my_e]) == to_float(row[e1]) && a.bias[my_e] == a.bias[e1]);
         }
-        if (__any_sync(0xffffffffu, doubt)) my_e = choose_exactly<L, PER>(row, a.bias, a.E, a.topk);
+        if (__any_sync(0xffffffffu, doubt))
+            my_e = n <= 32 && picks <= 32 ? rank_exactly(row, a.bias, found[0], n, a.topk) : choose_exactly<L, PER>(row, a.bias, a.E, a.topk);
     }
     const bool any = lane < a.topk && my_e >= 0;
     const float w = pick_weight(a, any, any ? to_float(row[my_e]) : 0.f, highest, denominator);
@@ -223,6 +307,11 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_bwd_kernel(RouteBwd a)
     if (t >= a.T) return;                                  // warp-uniform
     const L* row = (const L*)a.logits + (size_t)t * a.row_stride;
     L* out = (L*)a.dlogits + (size_t)t * a.E;
+    float rest[PER];                                       // gradients of the experts that were not chosen
+#pragma unroll
+    for (int i = 0; i < PER; ++i) rest[i] = 0.f;
+    const bool dense = a.softmax && !a.renorm;
+    if (!dense) store_run<L, PER>(out, lane * PER, a.E, a.vec, rest);      // (before anything has to be waited for)
     int e = -1;
     float g = 0.f, l = 0.f;
     if (lane < a.topk)
@@ -233,9 +322,6 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_bwd_kernel(RouteBwd a)
     }
     const bool any = e >= 0;
     float mine = 0.f;                                      // gradient of this lane's pick
-    float rest[PER];                                       // and of the experts that were not chosen
-#pragma unroll
-    for (int i = 0; i < PER; ++i) rest[i] = 0.f;
     if (a.renorm)
     {
         const float high = warp_max(any ? l : -INFINITY), m = a.softmax ? high : fminf(high, 0.f);
@@ -262,7 +348,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_bwd_kernel(RouteBwd a)
 #pragma unroll
         for (int i = 0; i < PER; ++i) rest[i] = -a.scale * (v[i] / s) * mean;
     }
-    store_run<L, PER>(out, lane * PER, a.E, a.vec, rest);
+    if (dense) store_run<L, PER>(out, lane * PER, a.E, a.vec, rest);
     __syncwarp();                                          // the chosen experts' values come on top of what other lanes wrote
     if (any) out[e] = from_float<L>(mine);
 }
