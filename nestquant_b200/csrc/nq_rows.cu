@@ -10,13 +10,14 @@
 // topk independent loads or stores are in flight per thread; the gradient of combine has whole CTAs or warps per token for the dot
 // products, eight picks at a time.
 #include <initializer_list>
+#include <type_traits>
 
 #include "nq_common.cuh"
 #include "nq_types.cuh"
 
 namespace nq {
 
-constexpr int kRowsThreads = 256;
+constexpr int kRowsThreads = 256, kPicks = 8;       // picks of a token at a time
 
 struct Rows {
     const void* src; void* dst;
@@ -82,6 +83,36 @@ __device__ __forceinline__ void store_piece(T* p, const float (&v)[N])
     }
 }
 
+// the same as zeros where `there` does not hold: no branch, so that the loads of several picks are on their way together
+template <class T, int N>
+struct Piece {
+    static constexpr int kBytes = N * (int)sizeof(T), kWords = kBytes < 4 ? 1 : kBytes / 4;
+    uint32_t w[kWords];
+    __device__ __forceinline__ void load(const T* p, bool there)
+    {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = 0;
+        if (kBytes >= 16)
+#pragma unroll
+            for (int i = 0; i < kWords; i += 4)
+                asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\t@p ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+                             : "+r"(w[i]), "+r"(w[(i + 1) % kWords]), "+r"(w[(i + 2) % kWords]), "+r"(w[(i + 3) % kWords]) : "l"((const char*)p + 4 * i), "r"((unsigned)there) : "memory");
+        else if (kBytes == 8)
+            asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %3, 0;\n\t@p ld.global.v2.u32 {%0, %1}, [%2];\n\t}" : "+r"(w[0]), "+r"(w[1 % kWords]) : "l"(p), "r"((unsigned)there) : "memory");
+        else if (kBytes == 4)
+            asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p ld.global.u32 %0, [%1];\n\t}" : "+r"(w[0]) : "l"(p), "r"((unsigned)there) : "memory");
+        else
+            asm volatile("{\n\t.reg .pred p;\n\t.reg .u16 h;\n\tsetp.ne.u32 p, %2, 0;\n\tmov.u16 h, 0;\n\t@p ld.global.u16 h, [%1];\n\tcvt.u32.u16 %0, h;\n\t}" : "=r"(w[0]) : "l"(p), "r"((unsigned)there) : "memory");
+    }
+    __device__ __forceinline__ float at(int j) const
+    {
+        if (sizeof(T) == 4) return __uint_as_float(w[j % kWords]);
+        const unsigned short h = (unsigned short)(w[j / 2 % kWords] >> (16 * (j & 1)));
+        if (std::is_same<T, __half>::value) return __half2float(__ushort_as_half(h));
+        return __uint_as_float((uint32_t)h << 16);
+    }
+};
+
 // dst[t] = sum over the token's picks of src[pos] (times rw): dx of dispatch, out of combine
 template <class S, class D, int N, bool WEIGHTED>
 __global__ void __launch_bounds__(kRowsThreads) sum_kernel(Rows a)
@@ -95,16 +126,22 @@ __global__ void __launch_bounds__(kRowsThreads) sum_kernel(Rows a)
     const size_t pick = t * a.topk;
     const S* src = (const S*)a.src + (size_t)v * N;
     float sum[N] = {};
-#pragma unroll 8
-    for (int k = 0; k < a.topk; ++k)
+    for (int k0 = 0; k0 < a.topk; k0 += kPicks)
     {
-        const int p = a.pos[pick + k];
-        if (p >= live) continue;
-        float x[N];
-        load_piece<S, N>(src + (size_t)p * a.H, x);
-        const float w = WEIGHTED ? load_as(a.rw, a.rw_type, pick + k) : 1.f;
+        int p[kPicks];
+        Piece<S, N> x[kPicks];
 #pragma unroll
-        for (int j = 0; j < N; ++j) sum[j] += w * x[j];
+        for (int k = 0; k < kPicks; ++k) p[k] = k0 + k < a.topk ? a.pos[pick + k0 + k] : 0x7fffffff;
+#pragma unroll
+        for (int k = 0; k < kPicks; ++k) x[k].load(src + (size_t)p[k] * a.H, p[k] < live);
+#pragma unroll
+        for (int k = 0; k < kPicks; ++k)
+        {
+            if (p[k] >= live) continue;
+            const float w = WEIGHTED ? load_as(a.rw, a.rw_type, pick + k0 + k) : 1.f;
+#pragma unroll
+            for (int j = 0; j < N; ++j) sum[j] += w * x[k].at(j);
+        }
     }
     store_piece<D, N>((D*)a.dst + t * a.H + (size_t)v * N, sum);
 }
@@ -120,11 +157,10 @@ struct CombineBwd {
 template <class Y, class O, int N>
 __global__ void __launch_bounds__(kRowsThreads) combine_bwd_kernel(CombineBwd a)
 {
-    constexpr int kPicks = 8;
     __shared__ float s_dot[kRowsThreads / 32][kPicks];
     const int per = 32 * a.warps, slot = threadIdx.x / per, r = threadIdx.x % per, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const size_t t = (size_t)blockIdx.x * (kRowsThreads / per) + slot;
-    const bool there = t < (size_t)a.T;                   // every thread passes the barriers
+    const bool there = t < (size_t)a.T;             // every thread passes the barriers
     const int live = *a.live;
     for (int k0 = 0; k0 < a.topk; k0 += kPicks)
     {
@@ -142,28 +178,27 @@ __global__ void __launch_bounds__(kRowsThreads) combine_bwd_kernel(CombineBwd a)
             for (int v = r; v < a.pieces; v += per)
             {
                 float d[N];
+                Piece<Y, N> y[kPicks];
+                if (a.drw)
+#pragma unroll
+                    for (int k = 0; k < kPicks; ++k) y[k].load((const Y*)a.y + (size_t)p[k] * a.H + (size_t)v * N, k < n && p[k] < live);
                 load_piece<O, N>((const O*)a.dout + t * a.H + (size_t)v * N, d);
+                if (a.dy)
 #pragma unroll
-                for (int k = 0; k < kPicks; ++k)
-                {
-                    if (k >= n) continue;
-                    const size_t o = (size_t)p[k] * a.H + (size_t)v * N;
-                    const bool lives = p[k] < live;
-                    if (a.drw && lives)
+                    for (int k = 0; k < kPicks; ++k)
                     {
-                        float y[N];
-                        load_piece<Y, N>((const Y*)a.y + o, y);
-#pragma unroll
-                        for (int j = 0; j < N; ++j) dot[k] += y[j] * d[j];
-                    }
-                    if (a.dy)
-                    {
+                        if (k >= n) continue;
                         float g[N];
 #pragma unroll
-                        for (int j = 0; j < N; ++j) g[j] = lives ? w[k] * d[j] : 0.f;
-                        store_piece<Y, N>((Y*)a.dy + o, g);
+                        for (int j = 0; j < N; ++j) g[j] = p[k] < live ? w[k] * d[j] : 0.f;
+                        store_piece<Y, N>((Y*)a.dy + (size_t)p[k] * a.H + (size_t)v * N, g);
                     }
-                }
+                if (a.drw)
+#pragma unroll
+                    for (int k = 0; k < kPicks; ++k)
+                        if (k < n && p[k] < live)
+#pragma unroll
+                            for (int j = 0; j < N; ++j) dot[k] += y[k].at(j) * d[j];
             }
         if (!a.drw) continue;
 #pragma unroll
@@ -174,25 +209,32 @@ __global__ void __launch_bounds__(kRowsThreads) combine_bwd_kernel(CombineBwd a)
             for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
             if (lane == 0) s_dot[warp][k] = s;
         }
-        __syncthreads();
+        if (a.warps == 1) __syncwarp();
+        else __syncthreads();
         if (r < n)
         {
             float s = 0.f;
             for (int q = 0; q < a.warps; ++q) s += s_dot[slot * a.warps + q][r];
             store_as(a.drw, a.rw_type, pick + r, s);
         }
-        __syncthreads();
+        if (a.warps == 1) __syncwarp();
+        else __syncthreads();
     }
 }
 
-// elements that can be moved at a time: 16 bytes of S if rows and pointers allow it, else one
+// the most elements, 16 bytes of S at most, that rows of H elements at these pointers can be moved by; a wider type's pieces are stored 16 bytes at a time
 template <class S>
-bool wide_rows(int H, std::initializer_list<const void*> ptrs)
+int row_step(int H, int widest, std::initializer_list<const void*> ptrs)
 {
-    if ((size_t)H * sizeof(S) % 16) return false;
-    for (const void* p : ptrs)
-        if (!aligned16(p)) return false;
-    return true;
+    int n = 16 / (int)sizeof(S);
+    for (; n > 1; n /= 2)
+    {
+        const size_t align = (size_t)n * widest < 16 ? (size_t)n * widest : 16;
+        bool fits = H % n == 0;
+        for (const void* p : ptrs) fits = fits && reinterpret_cast<uintptr_t>(p) % align == 0;
+        if (fits) break;
+    }
+    return n;
 }
 int row_grid(int T, int pieces, unsigned* grid, const char* what)
 {
@@ -205,12 +247,13 @@ int row_grid(int T, int pieces, unsigned* grid, const char* what)
 template <class S, class D, bool WEIGHTED>
 int sum_rows(Rows a, cudaStream_t st, const char* what)
 {
-    constexpr int kN = 16 / (int)sizeof(S);
-    const bool wide = wide_rows<S>(a.H, {a.src, a.dst});
-    a.pieces = wide ? a.H / kN : a.H;
+    const int n = row_step<S>(a.H, (int)(sizeof(D) > sizeof(S) ? sizeof(D) : sizeof(S)), {a.src, a.dst});
+    a.pieces = a.H / n;
     unsigned grid;
     if (int e = row_grid(a.T, a.pieces, &grid, what)) return e;
-    if (wide) sum_kernel<S, D, kN, WEIGHTED><<<grid, kRowsThreads, 0, st>>>(a);
+    if (n == 8) { if constexpr (sizeof(S) == 2) sum_kernel<S, D, 8, WEIGHTED><<<grid, kRowsThreads, 0, st>>>(a); }
+    else if (n == 4) sum_kernel<S, D, 4, WEIGHTED><<<grid, kRowsThreads, 0, st>>>(a);
+    else if (n == 2) sum_kernel<S, D, 2, WEIGHTED><<<grid, kRowsThreads, 0, st>>>(a);
     else sum_kernel<S, D, 1, WEIGHTED><<<grid, kRowsThreads, 0, st>>>(a);
     return check_launch(what);
 }
@@ -218,12 +261,15 @@ int sum_rows(Rows a, cudaStream_t st, const char* what)
 template <class Y, class O>
 int combine_bwd(CombineBwd a, cudaStream_t st)
 {
-    constexpr int kN = 16 / (int)sizeof(Y);
-    const bool wide = wide_rows<Y>(a.H, {a.dout, a.y, a.dy}) && (size_t)a.H * sizeof(O) % 16 == 0;
-    a.pieces = wide ? a.H / kN : a.H;
-    a.warps = a.pieces > 128 ? 8 : a.pieces > 64 ? 4 : a.pieces > 32 ? 2 : 1;
+    const int n = row_step<Y>(a.H, (int)(sizeof(O) > sizeof(Y) ? sizeof(O) : sizeof(Y)), {a.dout, a.y, a.dy});
+    a.pieces = a.H / n;
+    // a warp per token if that makes 16 for each SM; more where there are few tokens and rows are long
+    a.warps = 1;
+    while (a.warps < 8 && 32 * a.warps < a.pieces && (long long)a.T * a.warps < 2368) a.warps *= 2;
     const int tokens = kRowsThreads / (32 * a.warps), grid = (a.T - 1) / tokens + 1;
-    if (wide) combine_bwd_kernel<Y, O, kN><<<grid, kRowsThreads, 0, st>>>(a);
+    if (n == 8) { if constexpr (sizeof(Y) == 2) combine_bwd_kernel<Y, O, 8><<<grid, kRowsThreads, 0, st>>>(a); }
+    else if (n == 4) combine_bwd_kernel<Y, O, 4><<<grid, kRowsThreads, 0, st>>>(a);
+    else if (n == 2) combine_bwd_kernel<Y, O, 2><<<grid, kRowsThreads, 0, st>>>(a);
     else combine_bwd_kernel<Y, O, 1><<<grid, kRowsThreads, 0, st>>>(a);
     return check_launch("nq_combine_bwd");
 }
