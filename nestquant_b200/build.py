@@ -15,6 +15,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "libnestquant_b200.so")
+OPS = os.path.join(HERE, "_torch_ops.so")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr", "-Xptxas", "-v"]
 
@@ -24,6 +25,27 @@ def nvcc():
         if c and os.path.exists(c):
             return c
     raise RuntimeError("nvcc not found (set NVCC)")
+
+
+def _torch_ops(lib, force=False, verbose=False):
+    """nestquant_b200/_torch_ops.so, the torch side of routing.py and w4.py (host code only), linked against the library"""
+    src = os.path.join(CSRC, "torch_ops.cpp")
+    if not force and os.path.exists(OPS) and os.path.getmtime(OPS) >= max(os.path.getmtime(f) for f in (src, os.path.join(os.path.dirname(HERE), "include", "nestquant_b200.h"))):
+        return OPS
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension as X
+    inc = X.include_paths("cuda") + [sysconfig.get_paths()["include"]]
+    libs = X.library_paths("cuda")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_EXTENSION_NAME=_torch_ops"]
+    cmd += [f"-isystem{d}" for d in inc] + [src, "-o", OPS] + [f"-L{d}" for d in libs] + [f"-L{HERE}", "-l:" + os.path.basename(lib), "-Wl,-rpath,$ORIGIN"]
+    cmd += ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-lcudart"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if verbose:
+        print(r.stderr, file=sys.stderr)
+    if r.returncode:
+        raise RuntimeError("g++ failed for torch_ops.cpp:\n" + r.stderr[-4000:])
+    return OPS
 
 
 def sources():
@@ -53,15 +75,17 @@ def _compile(src, verbose):
 
 
 def build(force=False, verbose=False):
-    """Compile every csrc/*.cu and link the shared library.  Returns its path."""
+    """Compile every csrc/*.cu and link the shared library, and the torch module on top of it.  Returns the library's path."""
     os.makedirs(OBJ, exist_ok=True)
     if not force and os.path.exists(LIB) and os.path.getmtime(LIB) >= _newest_dep():
+        _torch_ops(LIB, force, verbose)
         return LIB
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
         objs = list(ex.map(lambda s: _compile(s, verbose), sources()))
     r = subprocess.run([nvcc()] + ARCH + ["-shared", "-o", LIB] + objs + ["-lcudart"], capture_output=True, text=True)
     if r.returncode:
         raise RuntimeError("link failed:\n" + r.stderr[-4000:])
+    _torch_ops(LIB, force, verbose)
     return LIB
 
 

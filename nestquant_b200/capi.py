@@ -156,20 +156,11 @@ def current_stream():
     return torch.cuda.current_stream().cuda_stream
 
 
-def element_types():
-    """torch dtype -> NQ_F32 / NQ_F16 / NQ_BF16"""
-    import torch
-    return {torch.float32: NQ_F32, torch.float16: NQ_F16, torch.bfloat16: NQ_BF16}
 
-
-def launch(what, f, t, *args):
-    """f(*args, stream), an entry point whose last argument is the stream, on t's device and that device's current stream"""
-    import torch
-    d = t.get_device()
-    if d == torch.cuda.current_device():
-        rc = f(*args, torch._C._cuda_getCurrentRawStream(d))
-    else:
-        with torch.cuda.device(d):
-            rc = f(*args, torch._C._cuda_getCurrentRawStream(d))
-    if rc:
-        check(rc, what)
+def torch_ops():
+    """The torch side of the calls around the routed experts (csrc/torch_ops.cpp), built beside the library"""
+    if not os.path.exists(os.path.join(HERE, "_torch_ops.so")):
+        raise NestQuantError(f"{HERE}/_torch_ops.so is missing: run `python -m nestquant_b200.build`; there is no CPU or PyTorch fallback for this path")
+    import torch  # noqa: F401  (its libraries)
+    from . import _torch_ops
+    return _torch_ops
