@@ -181,9 +181,11 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) w4_kernel(W4 a)
         }
         planes.ask(there, zeros);
     };
-    // the planes do not come from a kernel that lets its successors in early: those of a single matrix are asked for before the wait
+    // the planes do not come from a kernel that lets its successors in early: those of a single matrix are asked for before the wait.  Half of the ring
+    // first, then the rows of x, then the other half, which need not be there when the products begin.
+    constexpr int kDepth = Stream::kDepth, kBefore = kDepth / 2;
 #pragma unroll 1
-    for (int d = 0; d < Stream::kDepth; ++d) ask();
+    for (int d = 0; d < kBefore; ++d) ask();
     if (!a.start) grid_dependency_wait();
     launch_dependents();
     if (ck > 1) cluster_arrive();                       // the others' shared memory is there when all have come by
@@ -224,7 +226,13 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) w4_kernel(W4 a)
                     asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" :: "r"(to), "l"((const X*)a.x + (size_t)(base + r) * a.x_stride + (there ? k : 0)), "r"(there) : "memory");
             }
             copies_end();
-            copies_done<0>();                             // (and the units that were asked for before)
+            if (i == i0)
+            {
+#pragma unroll 1
+                for (int d = kBefore; d < kDepth; ++d) ask();
+                copies_done<kDepth - kBefore>();
+            }
+            else copies_done<0>();                        // (and the units that were asked for before)
             __syncthreads();
         }
         const uint32_t x0 = shared_address(s_x) + (u0 - c0) * 256;
@@ -309,7 +317,8 @@ bool w4_cut(W4& a, int rows, int device, cudaLaunchConfig_t& cfg, long long& clu
         for (int log_wk = 0; log_wk <= 4 && ck << log_wk <= a.C; ++log_wk)
         {
             const int blocks = (a.S - 1) / (kW4Warps >> log_wk) + 1, units = ((a.C - 1) >> (log_ck + log_wk)) + 1;
-            const double cost = (((long long)blocks * experts - 1) / there + 1) * (units + (ck > 1 ? 3.0 : 1.5));
+            // (16 units, one for each warp, come through the same door as 16 KB of x)
+            const double cost = (((long long)blocks * experts - 1) / there + 1) * (units + (ck > 1 ? 3.0 : 1.5)) + rows * w4_pitch(a.C, ck) / 16384.0;
             if (best == 0 || cost < best)
             {
                 best = cost;

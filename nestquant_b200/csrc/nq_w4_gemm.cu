@@ -28,7 +28,9 @@ struct WgPlan {
     static constexpr int kThreads = kSplit ? 640 : 32 * 26;
     static constexpr int kColumns = TOKENS / 2;                           // tokens of a sum warp
     using Stream = W4Stream<GROUPS, 4, kHalves>;
-    static constexpr int kStages = TOKENS == 128 ? 4 : 6;                 // chunks ahead; a weight tile is 64 columns of tensor memory
+    // groups whose sums are kept side by side in one of the two accumulators: the waits are per accumulator
+    static constexpr int kSet = GROUPS * TOKENS <= 128 ? GROUPS : 128 / TOKENS, kSumColumns = kSet * TOKENS;
+    static constexpr int kStages = kSumColumns == 128 ? 4 : 6;                 // chunks ahead; a weight tile is 64 columns of tensor memory
     static constexpr int kBox = TOKENS * 128;                             // a token tile of 64 columns
     static constexpr int kTiles = kStages * 2 * kBox, kPlanes = kDecodeWarps * Stream::kBytes, kSums = TOKENS * 512;
     // tiles, and after them, or in their place once they are through, the sums of a split item; planes
@@ -46,25 +48,27 @@ __device__ __forceinline__ void tma_two_boxes(uint32_t dst, uint32_t box, const 
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                  ::"r"(dst + box), "l"(map), "r"(x + 64), "r"(y), "r"(bar) : "memory");
 }
-// The MMAs of a group of STEPS steps of 16 columns and the commit to `full`, by one elected lane (one election, few instructions: this warp shares its scheduler
+// The MMAs of a group of STEPS steps of 16 columns and, with COMMIT, the commit to `full`, by one elected lane (one election, few instructions: this warp shares its scheduler
 // with busy ones).  Weights in tensor memory, 8 columns a step; tokens in shared memory, two tiles of 64 columns, BOX bytes apart (the descriptor counts in 16
 // bytes).  The first MMA overwrites the accumulator.
 #define NQ_WG_STEP(A, B, P) \
     "add.u32 ta, %1, " A ";\n\tadd.u32 tb, %2, " B ";\n\tmov.b64 db, {tb, %3};\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ta], db, %4, " P ";\n\t"
-#define NQ_WG_GROUP(STEPS_TEXT)                                                                                                                       \
+#define NQ_WG_GROUP(STEPS_TEXT, COMMIT)                                                                                                                       \
     asm volatile("{\n\t.reg .pred p, q, e;\n\t.reg .b64 db;\n\t.reg .b32 ta, tb;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 p, %4, %4;\n\tsetp.eq.u32 q, %4, %4;\n\t"  \
-                 STEPS_TEXT "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%5];\n\t}"                                     \
+                 STEPS_TEXT COMMIT "}"                                                                                                                 \
                  ::"r"(d), "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(full), "n"(BOX >> 4) : "memory")
-template <int STEPS, int BOX>
+#define NQ_WG_COMMIT "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%5];\n\t"
+#define NQ_WG_EITHER(STEPS_TEXT) do { if (COMMIT) NQ_WG_GROUP(STEPS_TEXT, NQ_WG_COMMIT); else NQ_WG_GROUP(STEPS_TEXT, ""); } while (0)
+template <int STEPS, int BOX, bool COMMIT>
 __device__ __forceinline__ void mma_group(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t full)
 {
     if constexpr (STEPS == 8)
-        NQ_WG_GROUP(NQ_WG_STEP("0", "0", "p") NQ_WG_STEP("8", "2", "q") NQ_WG_STEP("16", "4", "q") NQ_WG_STEP("24", "6", "q")
-                    NQ_WG_STEP("32", "%6", "q") NQ_WG_STEP("40", "%6+2", "q") NQ_WG_STEP("48", "%6+4", "q") NQ_WG_STEP("56", "%6+6", "q"));
+        NQ_WG_EITHER(NQ_WG_STEP("0", "0", "p") NQ_WG_STEP("8", "2", "q") NQ_WG_STEP("16", "4", "q") NQ_WG_STEP("24", "6", "q")
+                     NQ_WG_STEP("32", "%6", "q") NQ_WG_STEP("40", "%6+2", "q") NQ_WG_STEP("48", "%6+4", "q") NQ_WG_STEP("56", "%6+6", "q"));
     else if constexpr (STEPS == 4)
-        NQ_WG_GROUP(NQ_WG_STEP("0", "0", "p") NQ_WG_STEP("8", "2", "q") NQ_WG_STEP("16", "4", "q") NQ_WG_STEP("24", "6", "q"));
+        NQ_WG_EITHER(NQ_WG_STEP("0", "0", "p") NQ_WG_STEP("8", "2", "q") NQ_WG_STEP("16", "4", "q") NQ_WG_STEP("24", "6", "q"));
     else
-        NQ_WG_GROUP(NQ_WG_STEP("0", "0", "p") NQ_WG_STEP("8", "2", "q"));
+        NQ_WG_EITHER(NQ_WG_STEP("0", "0", "p") NQ_WG_STEP("8", "2", "q"));
 }
 __device__ __forceinline__ void tmem_ld16_async(uint32_t taddr, uint32_t (&v)[16])
 {
@@ -240,29 +244,33 @@ __global__ void __launch_bounds__((WgPlan<GROUPS, TOKENS>::kThreads), 1) w4_gemm
                     next[1][j] = c + 2 < c1 ? sc[16 * GROUPS + 2 * j] : 0;
                 }
 #pragma unroll
-                for (int j = 0; j < GROUPS; ++j)
+                for (int j0 = 0; j0 < GROUPS; j0 += Plan::kSet)
                 {
                     ok = ok && wait_bar(saddr(&sh.sum_full[acc.s]), acc.parity, &sh.waits);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint64_t s = two_floats(scales_of<SC>(scale[j]).x);
                     constexpr int kAtOnce = kColumns < 32 ? kColumns : 32;
 #pragma unroll
-                    for (int k0 = 0; k0 < kColumns; k0 += kAtOnce)
+                    for (int j = 0; j < Plan::kSet; ++j)
                     {
-                        uint32_t v[kAtOnce / 16][16];
+                        const uint64_t s = two_floats(scales_of<SC>(scale[j0 + j]).x);
 #pragma unroll
-                        for (int h = 0; h < kAtOnce / 16; ++h) tmem_ld16_async(from + acc.s * TOKENS + k0 + 16 * h, v[h]);
-#pragma unroll
-                        for (int h = 0; h < kAtOnce / 16; ++h) tmem_wait_ld(v[h]);
-                        if (k0 + kAtOnce == kColumns)
+                        for (int k0 = 0; k0 < kColumns; k0 += kAtOnce)
                         {
-                            tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(&sh.sum_empty[acc.s]);
-                        }
+                            uint32_t v[kAtOnce / 16][16];
 #pragma unroll
-                        for (int k = 0; k < kAtOnce / 2; ++k) fma_two(sum[k0 / 2 + k], s, v[k / 8][2 * k % 16], v[k / 8][2 * k % 16 + 1]);
+                            for (int h = 0; h < kAtOnce / 16; ++h) tmem_ld16_async(from + acc.s * Plan::kSumColumns + j * TOKENS + k0 + 16 * h, v[h]);
+#pragma unroll
+                            for (int h = 0; h < kAtOnce / 16; ++h) tmem_wait_ld(v[h]);
+                            if (k0 + kAtOnce == kColumns && j == Plan::kSet - 1)
+                            {
+                                tc_fence_before();
+                                __syncwarp();
+                                if (lane == 0) mbar_arrive(&sh.sum_empty[acc.s]);
+                            }
+#pragma unroll
+                            for (int k = 0; k < kAtOnce / 2; ++k) fma_two(sum[k0 / 2 + k], s, v[k / 8][2 * k % 16], v[k / 8][2 * k % 16 + 1]);
+                        }
                     }
                     acc.next();
                 }
@@ -317,7 +325,7 @@ __global__ void __launch_bounds__((WgPlan<GROUPS, TOKENS>::kThreads), 1) w4_gemm
         };
 #pragma unroll 1
         for (int d = 0; d < Stream::kDepth; ++d) ask();
-        const uint32_t to = tmem + ((uint32_t)(strip * 16) << 16) + 2 * TOKENS;
+        const uint32_t to = tmem + ((uint32_t)(strip * 16) << 16) + 2 * Plan::kSumColumns;
         Ring<kStages> stage;
         stage.s = half;
         uint32_t stored = 0;                              // barrier of the unit whose stores are on their way
@@ -410,17 +418,18 @@ __global__ void __launch_bounds__((WgPlan<GROUPS, TOKENS>::kThreads), 1) w4_gemm
         for (int u = (i1 - i0) * (c1 - c0); u > 0 && ok; --u)
         {
             ok = wait_bar(saddr(&sh.full_a[stage.s]), stage.parity, &sh.waits) && wait_bar(saddr(&sh.full_b[stage.s]), stage.parity, &sh.waits);
-            const uint32_t w = tmem + 2 * TOKENS + stage.s * 64, b_lo = b0 + stage.s * (2 * Plan::kBox >> 4);
+            const uint32_t w = tmem + 2 * Plan::kSumColumns + stage.s * 64, b_lo = b0 + stage.s * (2 * Plan::kBox >> 4);
             auto group = [&](auto j) {
                 constexpr int kSteps = 8 / GROUPS, kFirst = decltype(j)::value * kSteps;
                 if constexpr (kFirst < 8)
                 {
-                    ok = ok && wait_bar(saddr(&sh.sum_empty[acc.s]), acc.parity ^ 1u, &sh.waits);
+                    constexpr int kPlace = decltype(j)::value % Plan::kSet;      // in the accumulator
+                    if (kPlace == 0) ok = ok && wait_bar(saddr(&sh.sum_empty[acc.s]), acc.parity ^ 1u, &sh.waits);
                     if (!ok) return;
                     tc_fence_after();
-                    mma_group<kSteps, Plan::kBox>(tmem + acc.s * TOKENS, w + kFirst * 8, b_lo + (kFirst >> 2) * (Plan::kBox >> 4) + (kFirst & 3) * 2, b_hi, kDesc,
-                                                  saddr(&sh.sum_full[acc.s]));
-                    acc.next();
+                    mma_group<kSteps, Plan::kBox, kPlace == Plan::kSet - 1>(tmem + acc.s * Plan::kSumColumns + kPlace * TOKENS, w + kFirst * 8,
+                                                                             b_lo + (kFirst >> 2) * (Plan::kBox >> 4) + (kFirst & 3) * 2, b_hi, kDesc, saddr(&sh.sum_full[acc.s]));
+                    if (kPlace == Plan::kSet - 1) acc.next();
                 }
             };
             group(std::integral_constant<int, 0>()); group(std::integral_constant<int, 1>()); group(std::integral_constant<int, 2>()); group(std::integral_constant<int, 3>());
