@@ -325,7 +325,7 @@ int nq_route_bwd(const void* logits, int type, long long row_stride, const int64
                  int renorm, float scale, void* dlogits, void* stream);
 
 /* The sort of nq_pf_sort by expert id alone: bin E has the picks whose id is outside [0, E).  start [E + 2]; scratch int32
- * [nq_pf_sort_scratch_ints(T * topk, E)]. */
+ * [nq_pf_sort_scratch_ints(T * topk, E)]; pe and pt may both be NULL (dispatch and combine need neither). */
 int nq_sort_picks(const int64_t* sel, int T, int topk, int E, int32_t* pe, int32_t* pt, int32_t* pos, int32_t* start, int32_t* scratch, int scratch_ints,
                   void* stream);
 /* xs[pos[t][k]] = x[t] for picks in front of *live (= start + E of nq_sort_picks), zeros for those behind: all of xs [T * topk][H] is written.

@@ -23,6 +23,7 @@
 #include "nq_common.cuh"
 #include "nq_format.cuh"
 #include "nq_plan.cuh"
+#include "nq_cluster.cuh"
 
 namespace nq {
 
@@ -123,7 +124,9 @@ __device__ __forceinline__ void place_picks(int* nx, int b, int i, int topk, int
     __syncwarp();
     if (b >= 0 && rank == __popc(same) - 1) nx[b] = p + 1;                     // the last lane of each bin moves the bin on
     __syncwarp();
-    if (b >= 0) { pe[p] = b; pt[p] = i / topk; pos[i] = p; }
+    if (b < 0) return;
+    pos[i] = p;
+    if (pe) { pe[p] = b; pt[p] = i / topk; }      // (scattered: a store a pick)
 }
 
 // pass 3: place every pick.  Every CTA adds up the bin sizes itself (row 0 of hist); CTA 0 writes them out as start.
@@ -205,6 +208,92 @@ __global__ void __launch_bounds__(1024) sort_small_kernel(const int64_t* sel, co
     if (plan) plan_passes<true>(s_start, table, E, 0, P, plan, max_passes, s_warp);
 }
 
+// nq_sort_picks of up to 65,536 picks: the three passes in one launch of up to eight CTAs that hand their counts around.  A warp has a slice of
+// up to 256 consecutive picks; a CTA adds up its warps' counts, reads the other CTAs' through distributed shared memory and so knows what of each bin lies
+// in front of its own picks.  256 / 20,004 / 32,768 picks of 256 / 64 / 256 experts: 3.2 / 5.9 / 6.7 us; as one kernel of 32 warps or three of them 5.4 / 13.5 / 16.1.
+constexpr int kSortIdsCtas = 8, kSortIdsPicks = kSortIdsCtas * 32 * kSortSlice;
+__global__ void __launch_bounds__(1024) sort_ids_kernel(const int64_t* sel, int P, int E, int topk, int slice, int ctas, int* start, int* pe, int* pt, int* pos)
+{
+    launch_dependents();
+    grid_dependency_wait();
+    extern __shared__ int s_hist[];      // [warps][E + 1] counts, then next free places; [E + 1] the CTA's counts; [E + 2] all counts, then starts
+    __shared__ int s_warp[32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, nb = E + 1, rank = blockIdx.x;
+    const int i0 = (rank * warps + warp) * slice;
+    int* h = s_hist + warp * nb;
+    int *s_mine = s_hist + warps * nb, *s_start = s_mine + nb;
+    int bin[kSortSlice / 32];
+    for (int b = lane; b < nb; b += 32) h[b] = 0;
+#pragma unroll
+    for (int j = 0; j < kSortSlice / 32; ++j)
+    {
+        const int i = i0 + 32 * j + lane;
+        bool hit;
+        bin[j] = 32 * j < slice && i < P ? pick_bin(sel, nullptr, nullptr, E, i, &hit) : -1 - lane;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < kSortSlice / 32; ++j)
+        if (bin[j] >= 0) atomicAdd(h + bin[j], 1);
+    __syncthreads();
+    for (int b = threadIdx.x; b < nb; b += blockDim.x)
+    {
+        int run = 0;
+#pragma unroll 8
+        for (int w = 0; w < warps; ++w) { const int c = s_hist[w * nb + b]; s_hist[w * nb + b] = run; run += c; }
+        s_mine[b] = run;
+    }
+    if (ctas > 1) { cluster_arrive(); cluster_wait(); }
+    // counts of all CTAs; what lies in the CTAs before this one
+    for (int b = threadIdx.x; b < nb; b += blockDim.x)
+    {
+        const uint32_t at = (uint32_t)__cvta_generic_to_shared(s_mine + b);
+        int count[kSortIdsCtas], all = 0, before = 0;
+#pragma unroll
+        for (int r = 0; r < kSortIdsCtas; ++r)
+        {
+            count[r] = 0;
+            if (r < ctas) asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(count[r]) : "r"(ctas > 1 ? cluster_address(at, r) : at) : "memory");
+        }
+#pragma unroll
+        for (int r = 0; r < kSortIdsCtas; ++r) { all += count[r]; before += r < rank ? count[r] : 0; }
+        s_start[b] = all;
+        for (int w = 0; w < warps; ++w) s_hist[w * nb + b] += before;
+    }
+    if (ctas > 1) cluster_arrive();                                            // (nobody leaves while its counts are being read)
+    __syncthreads();
+    scan_bins<false>(s_start, nb, s_start, s_warp);
+    if (rank == 0)
+        for (int b = threadIdx.x; b <= nb; b += blockDim.x) start[b] = s_start[b];
+    for (int b = lane; b < nb; b += 32) h[b] += s_start[b];
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < kSortSlice / 32; ++j)
+        if (32 * j < slice) place_picks(h, bin[j], i0 + 32 * j + lane, topk, lane, pe, pt, pos);
+    if (ctas > 1) cluster_wait();
+}
+int sort_ids(const int64_t* sel, int P, int topk, int E, int32_t* pe, int32_t* pt, int32_t* pos, int32_t* start, cudaStream_t st)
+{
+    // eight to sixteen warps of one to eight steps of 32 picks, more only where slices would be too long: a CTA's counts are added up warp by warp
+    const int ctas = P <= 256 ? 1 : kSortIdsCtas;
+    int warps = (P + 32 * ctas - 1) / (32 * ctas);
+    warps = warps < 8 ? 8 : warps <= 16 || P <= 32768 ? (warps < 16 ? warps : 16) : 32;
+    const int slice = ((P + warps * ctas - 1) / (warps * ctas) + 31) / 32 * 32;
+    const size_t smem = sizeof(int) * ((size_t)(warps + 2) * (E + 1) + 1);
+    if (cudaFuncSetAttribute(sort_ids_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(int) * (34 * kSortMaxBins + 1))) != cudaSuccess)
+        return fail(NQ_ERR_CUDA, "nq_sort_picks: shared memory");
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = ctas; attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = 2;
+    cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(32 * warps); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    cudaLaunchKernelEx(&cfg, sort_ids_kernel, sel, P, E, topk, slice, ctas, (int*)start, (int*)pe, (int*)pt, (int*)pos);
+    return check_launch("nq_sort_picks");
+}
+
 // the sort, and the pass list of the whole window if plan is given
 int sort_pairs(const int64_t* sel, const void* rw, const int64_t* table, int T, int topk, int E, int32_t* pe, int32_t* pt, int32_t* pos, int32_t* start,
                int32_t* hits, int32_t* scratch, int scratch_ints, int32_t* plan, int plan_ints, void* stream)
@@ -215,8 +304,9 @@ int sort_pairs(const int64_t* sel, const void* rw, const int64_t* table, int T, 
     NQ_REQUIRE(start, "nq_pf_sort: null start array");
     cudaStream_t st = (cudaStream_t)stream;
     if (P == 0) return cudaMemsetAsync(start, 0, sizeof(int32_t) * (E + 2), st) == cudaSuccess ? NQ_OK : fail(NQ_ERR_CUDA, "nq_pf_sort: memset failed");
-    NQ_REQUIRE(sel && !rw == !table && pe && pt && pos && scratch, "nq_pf_sort: null pointer");
+    NQ_REQUIRE(sel && !rw == !table && !pe == !pt && (pe || !table) && pos && scratch, "nq_pf_sort: null pointer");
     NQ_REQUIRE(scratch_ints >= nq_pf_sort_scratch_ints(P, E), "nq_pf_sort: scratch needs %d ints", nq_pf_sort_scratch_ints(P, E));
+    if (!table && P <= kSortIdsPicks) return sort_ids(sel, P, topk, E, pe, pt, pos, start, st);
     const size_t small = sizeof(int) * (33 * (size_t)(E + 1) + 1);
     if (P <= kSortSmallPicks && small <= kSortSmallShared)
     {

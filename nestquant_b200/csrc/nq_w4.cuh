@@ -15,6 +15,7 @@
 #pragma once
 #include <type_traits>
 
+#include "nq_cluster.cuh"
 #include "nq_common.cuh"
 #include "nq_scan.cuh"
 #include "nq_types.cuh"
@@ -241,20 +242,6 @@ __device__ __forceinline__ void zero_rows_behind(const W4& a, int behind)
 {
     for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < (size_t)(a.rows - behind) * a.N; i += (size_t)gridDim.x * blockDim.x)
         store_as(a.out, a.out_type, (behind + i / a.N) * a.out_stride + i % a.N, 0.f);
-}
-
-// every thread of every CTA of the cluster arrives and waits
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ uint32_t cluster_address(uint32_t address, int rank)
-{
-    uint32_t there;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(address), "r"(rank));
-    return there;
-}
-__device__ __forceinline__ void cluster_store(uint32_t address, float x, float y)
-{
-    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" :: "r"(address), "f"(x), "f"(y) : "memory");
 }
 
 }  // namespace nq

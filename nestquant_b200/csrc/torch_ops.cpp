@@ -113,14 +113,26 @@ std::tuple<Tensor, Tensor> route(const Tensor& logits_, int64_t topk, const std:
 
 // ---- rows by expert and back ----------------------------------------------------------------------------------------------------
 
-// The picks of a call sorted by expert: one buffer of int32, start [E + 2], then pos, expert and token [P] of each place, then the sort's scratch
+// The picks of a call sorted by expert: one buffer of int32, start [E + 2], then pos [P], then the sort's scratch.  Expert and token of each place are
+// worked out when they are asked for: no call needs them, and in the sort they are scattered stores.
 struct Order : torch::CustomClassHolder {
     int64_t T, topk, E;
     Tensor buf;
     int64_t P() const { return T * topk; }
-    Tensor part(int64_t i) const { return buf.narrow(0, E + 2 + i * P(), P()); }
     Tensor start() const { return buf.narrow(0, 0, E + 1); }
-    Tensor pos() const { return part(0).view({T, topk}); }
+    Tensor flat() const { return buf.narrow(0, E + 2, P()); }
+    Tensor pos() const { return flat().view({T, topk}); }
+    Tensor token() const
+    {
+        const c10::cuda::CUDAGuard guard(buf.device());
+        const Tensor picks = at::arange(P(), buf.options());
+        return at::empty_like(picks).scatter_(0, flat().to(at::kLong), at::floor_divide(picks, topk));
+    }
+    Tensor expert() const
+    {
+        const c10::cuda::CUDAGuard guard(buf.device());
+        return at::bucketize(at::arange(P(), buf.options()), buf.narrow(0, 1, E), /*out_int32=*/true, /*right=*/true);
+    }
     const int32_t* live_ptr() const { return buf.data_ptr<int32_t>() + E; }
     const int32_t* pos_ptr() const { return buf.data_ptr<int32_t>() + E + 2; }
 };
@@ -131,15 +143,15 @@ OrderPtr sort_picks(const Tensor& sel_, int64_t E)
     on_gpu(sel_, 2, "sort_picks: sel");
     NQ_CHECK(sel_.scalar_type() == at::kLong, "sort_picks: sel, expected int64");
     const int64_t T = sel_.size(0), topk = sel_.size(1);
-    NQ_CHECK(E >= 1 && E <= 1024 && topk >= 1 && 3 * T * topk + E + 2 <= 0x7fffffff, "sort_picks: ", T, " x ", topk, " picks of ", E, " experts (to 1024)");
+    NQ_CHECK(E >= 1 && E <= 1024 && topk >= 1 && 2 * T * topk + E + 2 <= 0x7fffffff, "sort_picks: ", T, " x ", topk, " picks of ", E, " experts (to 1024)");
     const c10::cuda::CUDAGuard guard(sel_.device());
     const Tensor sel = sel_.contiguous();
     const int ints = nq_pf_sort_scratch_ints((int)(T * topk), (int)E);
     auto o = c10::make_intrusive<Order>();
     o->T = T; o->topk = topk; o->E = E;
-    o->buf = at::empty({E + 2 + 3 * T * topk + std::max(ints, 1)}, sel.options().dtype(at::kInt));
-    int32_t* start = o->buf.data_ptr<int32_t>(), *pos = start + E + 2, *pe = pos + T * topk, *pt = pe + T * topk, *scratch = pt + T * topk;
-    check(nq_sort_picks(sel.data_ptr<int64_t>(), (int)T, (int)topk, (int)E, pe, pt, pos, start, scratch, std::max(ints, 1), stream_of(sel)), "sort_picks");
+    o->buf = at::empty({E + 2 + T * topk + std::max(ints, 1)}, sel.options().dtype(at::kInt));
+    int32_t *start = o->buf.data_ptr<int32_t>(), *pos = start + E + 2, *scratch = pos + T * topk;
+    check(nq_sort_picks(sel.data_ptr<int64_t>(), (int)T, (int)topk, (int)E, nullptr, nullptr, pos, start, scratch, std::max(ints, 1), stream_of(sel)), "sort_picks");
     return o;
 }
 
@@ -324,7 +336,7 @@ PYBIND11_MODULE(_torch_ops, m)
         "picks without an expert begin); pos [T,topk], place of each pick; expert [P] (E: none) and token [P] of each place, P = T * topk.")
         .def_readonly("T", &Order::T).def_readonly("topk", &Order::topk).def_readonly("E", &Order::E).def_property_readonly("P", &Order::P)
         .def_property_readonly("start", &Order::start).def_property_readonly("pos", &Order::pos)
-        .def_property_readonly("expert", [](const Order& o) { return o.part(1); }).def_property_readonly("token", [](const Order& o) { return o.part(2); });
+        .def_property_readonly("expert", &Order::expert).def_property_readonly("token", &Order::token);
     py::class_<W4Planes, W4Ptr>(m, "W4Planes")
         .def_readonly("qw", &W4Planes::qw).def_readonly("sc", &W4Planes::sc).def_readonly("status", &W4Planes::status)
         .def_property_readonly("zp", [](const W4Planes& w) { return w.zp.defined() ? c10::optional<Tensor>(w.zp) : c10::nullopt; })
