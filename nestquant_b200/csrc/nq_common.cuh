@@ -4,6 +4,8 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include <atomic>
+
 #include "../../include/nestquant_b200.h"
 
 namespace nq {
@@ -45,6 +47,17 @@ inline void launch_dependent(void (*kernel)(P...), dim3 grid, dim3 block, size_t
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr; cfg.numAttrs = 1;
     cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+// a kernel's limit of dynamic shared memory, set once per device
+template <auto* KERNEL>
+inline bool allow_shared(int bytes, int device)
+{
+    static std::atomic<uint64_t> done{0};
+    const uint64_t bit = device >= 0 && device < 64 ? 1ull << device : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return true;
+    if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return true;
 }
 #endif
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

@@ -280,7 +280,8 @@ int sort_ids(const int64_t* sel, int P, int topk, int E, int32_t* pe, int32_t* p
     warps = warps < 8 ? 8 : warps <= 16 || P <= 32768 ? (warps < 16 ? warps : 16) : 32;
     const int slice = ((P + warps * ctas - 1) / (warps * ctas) + 31) / 32 * 32;
     const size_t smem = sizeof(int) * ((size_t)(warps + 2) * (E + 1) + 1);
-    if (cudaFuncSetAttribute(sort_ids_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(int) * (34 * kSortMaxBins + 1))) != cudaSuccess)
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || !allow_shared<sort_ids_kernel>((int)(sizeof(int) * (34 * kSortMaxBins + 1)), device))
         return fail(NQ_ERR_CUDA, "nq_sort_picks: shared memory");
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];

@@ -281,8 +281,8 @@ int w4_chunks(int K) { return (K - 1) / 128 + 1; }
 int w4_pitch(int C, int ck) { return ((C + ck - 1) / ck) * 256 + 64; }
 
 // clusters of ck CTAs that the device runs at a time, one CTA per SM
-template <class K>
-int w4_clusters(K* kernel, int ck, int sms, int device, cudaLaunchConfig_t& cfg)
+template <auto* KERNEL>
+int w4_clusters(int ck, int sms, int device, cudaLaunchConfig_t& cfg)
 {
     static std::atomic<int> known[16][4];
     if (ck == 1) return sms;
@@ -290,7 +290,7 @@ int w4_clusters(K* kernel, int ck, int sms, int device, cudaLaunchConfig_t& cfg)
     int n = at ? at->load(std::memory_order_relaxed) : 0;
     if (n) return n;
     cfg.gridDim = dim3(ck);
-    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) { cudaGetLastError(); n = 1; }
+    if (cudaOccupancyMaxActiveClusters(&n, KERNEL, &cfg) != cudaSuccess || n < 1) { cudaGetLastError(); n = 1; }
     if (at) at->store(n, std::memory_order_relaxed);
     return n;
 }
@@ -313,7 +313,7 @@ bool w4_cut(W4& a, int rows, int device, cudaLaunchConfig_t& cfg, long long& clu
         cudaLaunchAttribute& cluster = cfg.attrs[0];
         cluster.val.clusterDim.x = ck;
         cfg.dynamicSmemBytes = Plan::kPlanes + Plan::kParts + (size_t)rows * w4_pitch(a.C, ck);
-        const int there = w4_clusters(w4_kernel<X, SC, GROUPS, TILES>, ck, a.sms, device, cfg);
+        const int there = w4_clusters<w4_kernel<X, SC, GROUPS, TILES>>(ck, a.sms, device, cfg);
         for (int log_wk = 0; log_wk <= 4 && ck << log_wk <= a.C; ++log_wk)
         {
             const int blocks = (a.S - 1) / (kW4Warps >> log_wk) + 1, units = ((a.C - 1) >> (log_ck + log_wk)) + 1;
@@ -336,7 +336,7 @@ int w4_launch(W4 a, int device, cudaStream_t st)
     using Plan = W4Plan<GROUPS, TILES>;
     const int rows = a.rows < 8 * TILES ? a.rows : 8 * TILES;
     auto* kernel = w4_kernel<X, SC, GROUPS, TILES>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kW4MaxShared) != cudaSuccess) return fail(NQ_ERR_CUDA, "nq_w4_matmul: shared memory");
+    if (!allow_shared<w4_kernel<X, SC, GROUPS, TILES>>(kW4MaxShared, device)) return fail(NQ_ERR_CUDA, "nq_w4_matmul: shared memory");
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;

@@ -494,7 +494,7 @@ int wg_launch(Wg g, int device, cudaStream_t st)
     CUtensorMap map;
     if (int e = w4_x_map(&map, a, TOKENS, std::is_same<X, __nv_bfloat16>::value)) return e;
     auto* kernel = w4_gemm_kernel<X, SC, GROUPS, TOKENS>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Plan::kSmem) != cudaSuccess) return fail(NQ_ERR_CUDA, "nq_w4_matmul: shared memory");
+    if (!allow_shared<w4_gemm_kernel<X, SC, GROUPS, TOKENS>>(Plan::kSmem, device)) return fail(NQ_ERR_CUDA, "nq_w4_matmul: shared memory");
     a.blocks = (a.S - 1) / 8 + 1;
     const long long most = (long long)a.blocks * (a.start ? a.rows / TOKENS + (a.E < a.rows ? a.E : a.rows) : (a.rows - 1) / TOKENS + 1);
     NQ_REQUIRE(most <= 0x7fffffff / a.C, "nq_w4_matmul: %d rows are too many", a.rows);
