@@ -348,7 +348,8 @@ int nq_combine_bwd(const void* dout, int out_type, const void* y, int type, cons
  *   nq_w4_matmul  out[r] = W x[r] for x [rows][x_stride >= K] of `type` (NQ_F16 or NQ_BF16; rows start on 16 bytes), out [rows][out_stride >= N] of type
  *                 or NQ_F32.  start NULL: one matrix (E = 1) for all rows.  Else int32 [E + 1] on the device: matrix e for the rows start[e] to
  *                 start[e + 1] - 1 (start[0] = 0), zeros into the rows from start[E] on.  status: int32 [1] on the device, set to 1 if a
- *                 device-side wait timed out (bounded waits, 2 s; the outputs are then invalid). */
+ *                 device-side wait timed out (bounded waits, 2 s; the outputs are then invalid), to 2 if start falls anywhere (all rows are then
+ *                 zeros). */
 int nq_w4_units(int E, int N, int K, int64_t* units);
 int nq_w4_layout(const void* q, const void* scales, const void* zeros, int E, int N, int K, int group, void* qw, void* sc, void* zp, void* stream);
 int nq_w4_matmul(const void* x, int type, long long x_stride, const void* qw, const void* sc, int sc_type, const void* zp, const int32_t* start, int rows, int E,

@@ -84,11 +84,10 @@ __device__ __forceinline__ void unit_product(const W4Unit<GROUPS>& u, const uint
 // shared memory of a CTA
 template <int GROUPS, int TILES>
 struct W4Plan {
-    using Stream = W4Stream<GROUPS, TILES == 4 ? 3 : 4>;
+    using Stream = W4Stream<GROUPS, 4>;
     static constexpr int kPitch = 8 * TILES + 2, kPart = kW4Warps * 16 * kPitch;
-    // parts of two items, so that the sums of one wait for the next one's products; of one item where 32 rows leave no room
-    static constexpr int kBuffers = TILES == 4 ? 1 : 2;
-    static constexpr int kPlanes = kW4Warps * Stream::kBytes, kParts = kBuffers * kPart * 4, kRoom = kW4MaxShared - kPlanes - kParts;      // for rows of x
+    // parts of two items: the sums of one wait for the next one's products
+    static constexpr int kPlanes = kW4Warps * Stream::kBytes, kParts = 2 * kPart * 4, kRoom = kW4MaxShared - kPlanes - kParts;      // for rows of x
 };
 
 // A warp's share of an item: its part of the columns of one strip times the item's rows, while it asks for what comes kDepth units later
@@ -101,7 +100,7 @@ __device__ __forceinline__ void strip_product(STREAM& planes, int units, bool ze
 #pragma unroll
     for (int n = 0; n < TILES; ++n) xs[n] = x0 + min(8 * n + (lane >> 2), rows - 1) * pitch + (lane & 3) * 16;
     float sum[TILES][4] = {};
-#pragma unroll 2
+#pragma unroll 4
     for (int u = 0; u < units; ++u)
     {
         W4Unit<GROUPS> unit;
@@ -213,7 +212,7 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) w4_kernel(W4 a)
             // other rows of x: pieces of 128 columns, in turn to the warps
             pass = now.pass;
             base = s_row[now.e] + (pass - s_first[now.e]) * kRows;
-            rows = min(max(s_row[now.e + 1], s_row[now.e]) - base, kRows);
+            rows = min(s_row[now.e + 1] - base, kRows);
             __syncthreads();
             const int pieces = c1 - c0;
             for (int r = 0, c = warp; r < rows; c += kW4Warps)
@@ -237,13 +236,12 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) w4_kernel(W4 a)
         }
         const uint32_t x0 = shared_address(s_x) + (u0 - c0) * 256;
         float acc[TILES][4];
-        if (TILES >= 2 && rows <= 8) strip_product<X, SC, GROUPS, 1>(planes, units, zeros, x0, a.pitch, rows, lane, acc, ask);
-        else if (TILES == 4 && rows <= 16) strip_product<X, SC, GROUPS, 2>(planes, units, zeros, x0, a.pitch, rows, lane, acc, ask);
+        if (TILES == 2 && rows <= 8) strip_product<X, SC, GROUPS, 1>(planes, units, zeros, x0, a.pitch, rows, lane, acc, ask);
         else strip_product<X, SC, GROUPS, TILES>(planes, units, zeros, x0, a.pitch, rows, lane, acc, ask);
-        // two buffers: all parts of the item before this one are there, and those of the one before that have been read; one: they have been read
+        // all parts of the item before this one are there, and those of the one before that have been read
         if (i > i0 || ck > 1) barrier();
-        if (Plan::kBuffers == 2 && i > i0) add_up(s_part + ((i - 1) & 1) * Plan::kPart, old_block, old_base, old_rows);
-        const uint32_t to = shared_address(s_part + (Plan::kBuffers == 2 ? i & 1 : 0) * Plan::kPart);
+        if (i > i0) add_up(s_part + ((i - 1) & 1) * Plan::kPart, old_block, old_base, old_rows);
+        const uint32_t to = shared_address(s_part + (i & 1) * Plan::kPart);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
         {
@@ -254,21 +252,14 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) w4_kernel(W4 a)
                 if (q == 0 || 8 * q < rows) cluster_store(at + 32 * q, acc[q][2 * h], acc[q][2 * h + 1]);
         }
         if (ck > 1) cluster_arrive();
-        if (Plan::kBuffers == 1)
-        {
-            barrier();
-            add_up(s_part, now.block, base, rows);
-            if (ck > 1 && i + 1 < i1) cluster_arrive();
-        }
         old_block = now.block; old_base = base; old_rows = rows;
         now.next(blocks, s_first, a.E, passes);
     }
-    if (Plan::kBuffers == 1) return;
     barrier();
     add_up(s_part + ((i1 - 1) & 1) * Plan::kPart, old_block, old_base, old_rows);
 }
 
-int w4_gemm(const W4& a, int* status, int type, int sc_type, int group, int device, cudaStream_t st);       // nq_w4_gemm.cu
+int w4_gemm(const W4& a, int type, int sc_type, int group, int device, cudaStream_t st);       // nq_w4_gemm.cu
 
 bool w4_shape(int E, int N, int K, int g)
 {
@@ -360,11 +351,10 @@ int w4_launch(W4 a, int device, cudaStream_t st)
 template <class X, class SC, int GROUPS>
 int w4_tiles(const W4& a, int device, cudaStream_t st)
 {
-    // as many tiles of eight rows as the call has, or an expert on average; fewer where shared memory does not hold that many rows
-    const int pitch = w4_pitch(a.C, a.C < 8 ? a.C : 8), rows = a.start ? a.rows / a.E : a.rows;
-    if (rows <= 8 || 16 * pitch > W4Plan<GROUPS, 2>::kRoom) return w4_launch<X, SC, GROUPS, 1>(a, device, st);
-    if (rows <= 16 || 32 * pitch > W4Plan<GROUPS, 4>::kRoom) return w4_launch<X, SC, GROUPS, 2>(a, device, st);
-    return w4_launch<X, SC, GROUPS, 4>(a, device, st);
+    // one tile of eight rows where the call, or an expert on average, has no more, or shared memory does not hold sixteen; else two
+    const int rows = a.start ? a.rows / a.E : a.rows;
+    if (rows <= 8 || 16 * w4_pitch(a.C, a.C < 8 ? a.C : 8) > W4Plan<GROUPS, 2>::kRoom) return w4_launch<X, SC, GROUPS, 1>(a, device, st);
+    return w4_launch<X, SC, GROUPS, 2>(a, device, st);
 }
 template <class X, class SC>
 int w4_groups(const W4& a, int g, int device, cudaStream_t st)
@@ -405,13 +395,13 @@ int nq_w4_matmul(const void* x, int type, long long x_stride, const void* qw, co
     if (rows == 0) return NQ_OK;
     NQ_REQUIRE(x && qw && sc && out && status, "nq_w4_matmul: null pointer");
     NQ_REQUIRE(nq::aligned16(x) && x_stride % 8 == 0 && nq::aligned16(qw) && nq::aligned16(sc), "nq_w4_matmul: rows of x and planes start on 16 bytes");
-    nq::W4 a{(const uint4*)qw, (const uint16_t*)sc, (const uint8_t*)zp, x, start, out, x_stride, out_stride, rows, N, K, E, nq::w4_strips(N), nq::w4_chunks(K),
+    nq::W4 a{(const uint4*)qw, (const uint16_t*)sc, (const uint8_t*)zp, x, start, out, status, x_stride, out_stride, rows, N, K, E, nq::w4_strips(N), nq::w4_chunks(K),
              out_type, 0, 0, 0, 0, 0};
     int device;
     if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&a.sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
         return nq::fail(NQ_ERR_CUDA, "nq_w4_matmul: no device");
     cudaStream_t st = (cudaStream_t)stream;
-    if (nq::w4_many_rows(rows, E, start)) return nq::w4_gemm(a, status, type, sc_type, group, device, st);
+    if (nq::w4_many_rows(rows, E, start)) return nq::w4_gemm(a, type, sc_type, group, device, st);
     if (type == NQ_F16) return sc_type == NQ_F16 ? nq::w4_groups<__half, __half>(a, group, device, st) : nq::w4_groups<__half, __nv_bfloat16>(a, group, device, st);
     return sc_type == NQ_F16 ? nq::w4_groups<__nv_bfloat16, __half>(a, group, device, st) : nq::w4_groups<__nv_bfloat16, __nv_bfloat16>(a, group, device, st);
 }

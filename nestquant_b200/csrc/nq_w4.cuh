@@ -28,7 +28,7 @@ constexpr int kW4MaxColumns = 32768;          // eight rows of x in a cluster of
 
 struct W4 {
     const uint4* qw; const uint16_t* sc; const uint8_t* zp;
-    const void* x; const int* start; void* out;
+    const void* x; const int* start; void* out; int* status;
     long long x_stride, out_stride;
     int rows, N, K, E, S, C, out_type;
     int log_ck, log_wk, pitch, blocks, sms;         // see w4_kernel
@@ -221,27 +221,30 @@ struct W4Cursor {
     }
 };
 
-// The experts' rows and, with `rows` rows a pass, their first passes: row[0 .. E], first[0 .. E] in shared memory; all passes are returned.  Whole CTA,
-// kW4MaxExperts / 2 threads at least.  Whatever is in start, rows stay inside x and out.
+// The experts' rows and, with ROWS rows a pass, their first passes: row[0 .. E], first[0 .. E] in shared memory; all passes are returned.  Whole CTA,
+// kW4MaxExperts / 2 threads at least.  Whatever is in start, rows stay inside x and out: an array that falls anywhere is taken for one of empty experts,
+// and the status says so.
 template <int ROWS>
 __device__ __forceinline__ int expert_passes(const W4& a, int* row, int* first, int* s_warp)
 {
     auto at = [&](int e) { return e == 0 ? 0 : min(max(a.start[min(e, a.E)], 0), a.rows); };
     const int e0 = min(2 * (int)threadIdx.x, a.E), x0 = at(e0), x1 = at(e0 + 1), x2 = at(e0 + 2);
     const int n0 = e0 < a.E ? (max(x1 - x0, 0) + ROWS - 1) / ROWS : 0, n1 = e0 + 1 < a.E ? (max(x2 - x1, 0) + ROWS - 1) / ROWS : 0;
+    const bool falls = __syncthreads_or(x1 < x0 || x2 < x1);
     int passes;
-    const int before = cta_exclusive_sum(n0 + n1, s_warp, passes);
-    if (threadIdx.x == 0) { first[a.E] = passes; row[a.E] = at(a.E); }
-    if (e0 < a.E) { first[e0] = before; row[e0] = x0; }
-    if (e0 + 1 < a.E) { first[e0 + 1] = before + n0; row[e0 + 1] = x1; }
+    const int before = cta_exclusive_sum(falls ? 0 : n0 + n1, s_warp, passes);
+    if (threadIdx.x == 0) { first[a.E] = passes; row[a.E] = falls ? 0 : at(a.E); }
+    if (e0 < a.E) { first[e0] = before; row[e0] = falls ? 0 : x0; }
+    if (e0 + 1 < a.E) { first[e0 + 1] = before + (falls ? 0 : n0); row[e0 + 1] = falls ? 0 : x1; }
+    if (falls && blockIdx.x == 0 && threadIdx.x == 0) *a.status = 2;
     __syncthreads();
     return passes;
 }
 // zeros into the rows that no expert has
 __device__ __forceinline__ void zero_rows_behind(const W4& a, int behind)
 {
-    for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < (size_t)(a.rows - behind) * a.N; i += (size_t)gridDim.x * blockDim.x)
-        store_as(a.out, a.out_type, (behind + i / a.N) * a.out_stride + i % a.N, 0.f);
+    for (int r = behind + (int)blockIdx.x; r < a.rows; r += gridDim.x)
+        for (int n = threadIdx.x; n < a.N; n += blockDim.x) store_as(a.out, a.out_type, (size_t)r * a.out_stride + n, 0.f);
 }
 
 }  // namespace nq

@@ -140,7 +140,6 @@ __device__ __forceinline__ void cluster_meet()
 
 struct Wg {
     W4 w;
-    int* status;
     int log_ck;
 };
 
@@ -165,7 +164,7 @@ __global__ void __launch_bounds__((WgPlan<GROUPS, TOKENS>::kThreads), 1) w4_gemm
     if (saddr(wg_smem) & 1023u)          // (never: the swizzled tiles would be read from the wrong places)
     {
         grid_dependency_wait();
-        if (threadIdx.x == 0) atomicExch(g.status, 1);
+        if (threadIdx.x == 0) atomicExch(a.status, 1);
         return;
     }
     const int c0 = (rank * a.C) >> g.log_ck, c1 = ((rank + 1) * a.C) >> g.log_ck, blocks = a.blocks;
@@ -206,7 +205,7 @@ __global__ void __launch_bounds__((WgPlan<GROUPS, TOKENS>::kThreads), 1) w4_gemm
     // rows of x of an item
     auto rows_of = [&](const W4Cursor& c, int& base) {
         base = sh.row[c.e] + (c.pass - sh.first[c.e]) * TOKENS;
-        return min(max(sh.row[c.e + 1], sh.row[c.e]) - base, TOKENS);
+        return min(sh.row[c.e + 1] - base, TOKENS);
     };
     constexpr int kColumns = Plan::kColumns;
     if (warp < Plan::kSumWarps)
@@ -469,7 +468,7 @@ __global__ void __launch_bounds__((WgPlan<GROUPS, TOKENS>::kThreads), 1) w4_gemm
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (sh.waits.aborted && threadIdx.x == 0) atomicExch(g.status, 1);
+    if (sh.waits.aborted && threadIdx.x == 0) atomicExch(a.status, 1);
     if (warp == Plan::kMma) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
@@ -527,9 +526,9 @@ int wg_groups(const Wg& g, int group, int device, cudaStream_t st)
     return group == 128 ? wg_tokens<X, SC, 1>(g, device, st) : group == 64 ? wg_tokens<X, SC, 2>(g, device, st) : wg_tokens<X, SC, 4>(g, device, st);
 }
 
-int w4_gemm(const W4& a, int* status, int type, int sc_type, int group, int device, cudaStream_t st)
+int w4_gemm(const W4& a, int type, int sc_type, int group, int device, cudaStream_t st)
 {
-    const Wg g{a, status, 0};
+    const Wg g{a, 0};
     if (type == NQ_F16) return sc_type == NQ_F16 ? wg_groups<__half, __half>(g, group, device, st) : wg_groups<__half, __nv_bfloat16>(g, group, device, st);
     return sc_type == NQ_F16 ? wg_groups<__nv_bfloat16, __half>(g, group, device, st) : wg_groups<__nv_bfloat16, __nv_bfloat16>(g, group, device, st);
 }

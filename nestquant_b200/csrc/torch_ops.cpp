@@ -5,6 +5,7 @@
 // tensors' device.  Errors are thrown as nestquant_b200.capi.NestQuantError before anything is enqueued.
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include "../../include/nestquant_b200.h"
@@ -42,7 +43,15 @@ void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_
 Tensor strided(const Tensor& t) { return t.numel() == 0 || (t.stride(1) == 1 && t.stride(0) >= t.size(1)) ? t : t.contiguous(); }
 int64_t stride_of(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 bool wants_grad(const Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
-void once(const Tensor& grad) { NQ_CHECK(!(at::GradMode::is_enabled() && grad.defined() && grad.requires_grad()), "gradients of gradients: not built"); }
+// gradients that say so when somebody wants to differentiate them
+variable_list once(variable_list grads)
+{
+    if (!at::GradMode::is_enabled()) return grads;
+    const int n = (int)grads.size();
+    for (Tensor& g : grads)
+        if (g.defined()) g.requires_grad_(true);
+    return (*std::make_shared<torch::autograd::DelayedError>("nestquant_b200: gradients of gradients are not built", n))(std::move(grads));
+}
 
 // ---- route ----------------------------------------------------------------------------------------------------------------------
 
@@ -74,16 +83,15 @@ struct Route : torch::autograd::Function<Route> {
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
         if (!grads[1].defined()) return {Tensor(), Tensor(), Tensor()};
-        once(grads[1]);
         const variable_list saved = ctx->get_saved_variables();
-        const Tensor &logits = saved[0], &sel = saved[1], drw = grads[1].contiguous();
+        const Tensor logits = saved[0].detach(), &sel = saved[1], drw = grads[1].detach().contiguous();
         const c10::cuda::CUDAGuard guard(logits.device());
         Tensor grad = at::empty(logits.sizes(), logits.options());
         check(nq_route_bwd(logits.data_ptr(), type_of(logits.scalar_type(), "route"), stride_of(logits), sel.data_ptr<int64_t>(), drw.data_ptr(),
                            type_of(drw.scalar_type(), "route"), (int)logits.size(0), (int)logits.size(1), (int)ctx->saved_data["topk"].toInt(),
                            (int)ctx->saved_data["score"].toInt(), ctx->saved_data["renorm"].toBool(), (float)ctx->saved_data["scale"].toDouble(), grad.data_ptr(),
                            stream_of(logits)), "route backward");
-        return {grad, Tensor(), Tensor()};
+        return once({grad, Tensor(), Tensor()});
     }
 };
 
@@ -172,15 +180,14 @@ struct Dispatch : torch::autograd::Function<Dispatch> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
-        once(grads[0]);
         const auto held = ctx->saved_data["order"].toCapsule();
         const Order& o = static_cast<const Order&>(*held);
-        const Tensor dxs = grads[0].contiguous();
+        const Tensor dxs = grads[0].detach().contiguous();
         const c10::cuda::CUDAGuard guard(dxs.device());
         Tensor dx = at::empty({o.T, dxs.size(1)}, dxs.options());
         check(nq_dispatch_bwd(dxs.data_ptr(), type_of(dxs.scalar_type(), "dispatch"), o.pos_ptr(), o.live_ptr(), (int)o.T, (int)o.topk, (int)dxs.size(1), dx.data_ptr(), stream_of(dxs)),
               "dispatch backward");
-        return {dx, Tensor()};
+        return once({dx, Tensor()});
     }
 };
 
@@ -212,9 +219,8 @@ struct Combine : torch::autograd::Function<Combine> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
-        once(grads[0]);
         const variable_list saved = ctx->get_saved_variables();
-        const Tensor &y = saved[0], &rw = saved[1], dout = grads[0].contiguous();
+        const Tensor &y = saved[0], &rw = saved[1], dout = grads[0].detach().contiguous();
         const auto held = ctx->saved_data["order"].toCapsule();
         const Order& o = static_cast<const Order&>(*held);
         const c10::cuda::CUDAGuard guard(y.device());
@@ -224,7 +230,7 @@ struct Combine : torch::autograd::Function<Combine> {
         check(nq_combine_bwd(dout.data_ptr(), type_of(dout.scalar_type(), "combine"), y.data_ptr(), type_of(y.scalar_type(), "combine"), rw.data_ptr(),
                              type_of(rw.scalar_type(), "combine"), o.pos_ptr(), o.live_ptr(), (int)o.T, (int)o.topk, (int)y.size(1), dy.defined() ? dy.data_ptr() : nullptr,
                              drw.defined() ? drw.data_ptr() : nullptr, stream_of(y)), "combine backward");
-        return {dy, drw, Tensor(), Tensor()};
+        return once({dy, drw, Tensor(), Tensor()});
     }
 };
 

@@ -30,7 +30,8 @@ class W4:
         return _ops.w4_matmul(s._planes, x, start, dtype)
 
     def status(s):
-        """0, or 1 if a device-side wait of a call has run out (its results are then invalid).  Synchronises."""
+        """0; 1 if a device-side wait of a call has run out (its results are then invalid); 2 if a call was given a start that falls (its rows
+        are then zeros).  Synchronises."""
         return int(s._planes.status.item())
 
     def nbytes(s):

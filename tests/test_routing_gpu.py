@@ -216,7 +216,7 @@ def places(sel, E):
     return torch.tensor(order, dtype=torch.int64), live, torch.tensor(start, dtype=torch.int32)
 
 
-@pytest.mark.parametrize("T,E,topk", [(1, 1, 1), (3, 5, 2), (40, 64, 4), (2000, 7, 4), (32, 256, 8), (300, 1024, 31), (3000, 200, 3)])
+@pytest.mark.parametrize("T,E,topk", [(1, 1, 1), (3, 5, 2), (40, 64, 4), (2000, 7, 4), (32, 256, 8), (300, 1024, 31), (3000, 200, 3), (64, 33, 4), (65, 33, 4), (8191, 17, 8), (20000, 300, 4)])
 def test_sort_picks(T, E, topk):
     from nestquant_b200 import routing
     sel = picks(T, E, topk)
@@ -361,6 +361,42 @@ def test_a_training_step_captured_and_replayed():
         got = [t.clone() for t in held]
         for a, b in zip(got, step()):
             assert torch.equal(a, b)
+
+
+def test_gradients_cannot_be_differentiated_again():
+    from nestquant_b200 import routing
+    l = logits_of(6, 16).requires_grad_(True)
+    x = torch.randn(6, 32, device="cuda", requires_grad=True)
+    sel, rw = routing.route(l, 2, dtype=F32)
+    o = routing.sort_picks(sel, 16)
+    out = routing.combine(routing.dispatch(x, o).square(), o, rw)
+    gl, gx = torch.autograd.grad(out.square().sum(), (l, x), create_graph=True)
+    once = torch.autograd.grad(routing.combine(routing.dispatch(x, o).square(), o, routing.route(l, 2, dtype=F32)[1]).square().sum(), (l, x))
+    assert torch.equal(gl, once[0]) and torch.equal(gx, once[1])
+    for g in (gl, gx):
+        with pytest.raises(RuntimeError):
+            g.sum().backward(retain_graph=True)
+
+
+def test_unused_outputs_and_frozen_inputs():
+    from nestquant_b200 import routing
+    l = logits_of(6, 16).requires_grad_(True)
+    sel, rw = routing.route(l, 2, dtype=F32)
+    assert not sel.requires_grad and rw.requires_grad
+    with torch.no_grad():
+        assert not routing.route(l, 2)[1].requires_grad
+    o = routing.sort_picks(sel, 16)
+    y = torch.randn(12, 8, device="cuda")
+    out = routing.combine(y, o, rw)
+    out.sum().backward()
+    assert l.grad is not None and y.grad is None
+    l2 = logits_of(6, 16).requires_grad_(True)
+    _, rw2 = routing.route(l2, 2, dtype=F32)
+    l2.data.add_(0)
+    with torch.no_grad():
+        l2.add_(1)                                             # changed behind the backward pass: torch says so
+    with pytest.raises(RuntimeError):
+        rw2.sum().backward()
 
 
 def test_repeats_have_the_same_bits():

@@ -74,7 +74,7 @@ def rows_of(sizes, E, extra=0):
     return start, int(start[-1]) + extra
 
 
-@pytest.mark.parametrize("sizes,extra", [([0, 0, 0, 0, 0], 0), ([0, 0, 0, 0, 0], 3), ([1, 0, 2, 0, 1], 0), ([5, 8, 9, 0, 33], 7), ([0, 0, 0, 70, 0], 1), ([16, 17, 1, 3, 32], 40), ([200, 1, 130, 0, 64], 0)])
+@pytest.mark.parametrize("sizes,extra", [([0, 0, 0, 0, 0], 0), ([0, 0, 0, 0, 0], 3), ([1, 0, 2, 0, 1], 0), ([5, 8, 9, 0, 33], 7), ([0, 0, 0, 70, 0], 1), ([16, 17, 1, 3, 32], 40), ([30, 40, 20, 31, 29], 2), ([200, 1, 130, 0, 64], 0)])
 @pytest.mark.parametrize("N,K,g,dtype,out,zeros", [(48, 256, 128, F16, F16, False), (100, 352, 32, BF16, F32, True), (257, 1024, 64, BF16, BF16, True)])
 def test_a_matrix_per_expert(sizes, extra, N, K, g, dtype, out, zeros):
     from nestquant_b200 import w4
@@ -125,6 +125,107 @@ def test_values_that_are_not_finite_stay_in_their_rows():
     keep = [r for r in range(12) if r not in (3, 4)]
     assert torch.equal(y[keep].nan_to_num(), clean[keep].nan_to_num()) and y[4].isnan().all() and y[3, 5] == float("inf")
     assert not y[keep][:, [n for n in range(64) if n != 7]].isnan().any()
+
+
+@pytest.mark.parametrize("T", [20, 150])
+def test_values_that_are_not_finite_stay_in_their_rows_of_a_large_call(T):
+    from nestquant_b200 import w4
+    q, s, z = make(200, 512, 64, BF16)
+    w, x = w4.W4(q, s, z), torch.randn(T, 512, device="cuda").bfloat16()
+    clean = w(x)
+    x[T - 1, 300] = float("nan")
+    x[2, 5] = float("inf")
+    y = w(x)
+    keep = [r for r in range(T) if r not in (2, T - 1)]
+    assert torch.equal(y[keep], clean[keep]) and y[T - 1].isnan().all()
+    qe, se, ze = make(200, 512, 64, BF16, E=2)             # the next expert's rows are in the same tile
+    we, start = w4.W4(qe, se, ze), torch.tensor([0, T - 1, T], dtype=torch.int32, device="cuda")
+    x[2, 5] = 0
+    y = we(x, start=start)
+    assert not y[:T - 1].isnan().any() and y[T - 1].isnan().all()
+
+
+@pytest.mark.parametrize("T", [3, 16, 40])
+def test_long_rows_and_few_columns_of_the_result(T):
+    from nestquant_b200 import w4
+    for N, K, g in ((24, 20480, 128), (7, 32768, 64), (33, 12320, 32)):
+        q, s, z = make(N, K, g)
+        x = torch.randn(T, K, device="cuda").half()
+        check(w4.W4(q, s, z)(x, dtype=F32), x, dense(q, s, z, g), K)
+
+
+def test_many_experts():
+    from nestquant_b200 import w4
+    E, N, K = 1024, 20, 128
+    q, s, z = make(N, K, 32, E=E)
+    w = w4.W4(q, s, z)
+    for rows in ((torch.arange(E) % 7 == 0).int(), torch.full((E,), 2), torch.randint(0, 60, (E,), generator=torch.Generator().manual_seed(1))):
+        start = torch.cat([torch.zeros(1), rows.cumsum(0)]).int().cuda()
+        x = torch.randn(int(start[-1]), K, device="cuda").half()
+        y = w(x, start=start, dtype=F32)
+        W = dense(q, s, z, 32)
+        e = torch.repeat_interleave(torch.arange(E), rows.long()).cuda()
+        want = torch.einsum("pk,pnk->pn", x.double(), W[e])
+        size = torch.einsum("pk,pnk->pn", x.double().abs(), W[e].abs())
+        assert ((y.double() - want).abs() <= 40 * 2.0 ** -23 * size + 2.0 ** -24 * want.abs()).all()
+
+
+def test_a_start_that_falls_gives_zeros_and_says_so():
+    from nestquant_b200 import w4
+    for T in (9, 200):
+        q, s, z = make(48, 256, 64, E=4)
+        w, x = w4.W4(q, s, z), torch.randn(T, 256, device="cuda").half()
+        good = torch.tensor([0, 2, 5, 5, T], dtype=torch.int32, device="cuda")
+        y = w(x, start=good)
+        assert w.status() == 0
+        for bad in ([0, 5, 2, 5, T], [0, 2, 5, -1, T], [0, 2 ** 30, 3, 4, 5]):
+            assert (w(x, start=torch.tensor(bad, dtype=torch.int32, device="cuda")) == 0).all()
+            assert w.status() == 2
+        assert torch.equal(w(x, start=good), y)
+        over = torch.tensor([0, 2, 5, 5, 2 ** 30], dtype=torch.int32, device="cuda")      # ends behind the last row
+        assert torch.equal(w(x, start=over), y)
+
+
+def test_large_calls_on_two_streams_at_once():
+    from nestquant_b200 import w4
+    q, s, z = make(640, 1024, 128)
+    w, W = w4.W4(q, s, z), dense(q, s, z, 128)
+    xs = [torch.randn(T, 1024, device="cuda").half() for T in (40, 300)]
+    torch.cuda.synchronize()
+    streams, ys = [torch.cuda.Stream() for _ in xs], []
+    for _ in range(5):
+        for st, x in zip(streams, xs):
+            with torch.cuda.stream(st):
+                ys.append((w(x), x))
+    torch.cuda.synchronize()
+    for y, x in ys:
+        check(y, x, W, 1024)
+    assert w.status() == 0
+
+
+def test_the_first_calls_of_a_process_can_be_captured():
+    import subprocess
+    import sys
+    code = """
+import torch
+from nestquant_b200 import routing, w4
+q = torch.randint(0, 256, (64, 128), device="cuda", dtype=torch.uint8)
+w = w4.W4(q, torch.full((64, 4), 0.5, device="cuda", dtype=torch.float16))
+x, l = torch.ones(20, 256, device="cuda", dtype=torch.float16), torch.randn(20, 16, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    few, many = w(x[:3].clone()), w(x)
+    sel, rw = routing.route(l, 4)
+    o = routing.sort_picks(sel, 16)
+    out = routing.combine(routing.dispatch(x, o), o, rw, dtype=torch.float32)
+g.replay()
+torch.cuda.synchronize()
+assert torch.equal(few, many[:3]) and (out - 1).abs().max() < 4 * 2.0 ** -11, (few, out)      # weights of 16 bits that add up to 1
+print("captured")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
 
 
 def test_large_sums_stay_in_32_bits():
