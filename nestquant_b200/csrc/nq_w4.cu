@@ -1,6 +1,7 @@
 // Products with 4-bit weights (nq_w4.cuh): the layout of the planes, and the kernel for calls of few rows.
 #include <atomic>
 
+#include "nq_tc.cuh"
 #include "nq_w4.cuh"
 
 namespace nq {
@@ -132,7 +133,7 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) w4_kernel(W4 a)
     __shared__ int s_row[kW4MaxExperts + 1], s_first[kW4MaxExperts + 2], s_warp[32];       // experts' rows of x, first passes
     float* const s_part = reinterpret_cast<float*>(s_planes + Plan::kPlanes);
     char* const s_x = s_planes + Plan::kPlanes + Plan::kParts;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int lane = threadIdx.x & 31, warp = (int)uniform(threadIdx.x >> 5), g = lane >> 2, t = lane & 3;
     const int ck = 1 << a.log_ck, wk = 1 << a.log_wk, ws = kW4Warps >> a.log_wk, log_parts = a.log_ck + a.log_wk, blocks = a.blocks;
     const int rank = blockIdx.x & (ck - 1), w = warp & (wk - 1), in_block = warp >> a.log_wk, p = (rank << a.log_wk) + w;
     const int u0 = (p * a.C) >> log_parts, units = (((p + 1) * a.C) >> log_parts) - u0;

@@ -123,10 +123,10 @@ __device__ __forceinline__ void load_shared(uint32_t at, uint32_t (&v)[WORDS])
     else asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1 % WORDS]), "=r"(v[2 % WORDS]), "=r"(v[3 % WORDS]) : "r"(at));
 }
 template <int BYTES>
-__device__ __forceinline__ void copy_async(uint32_t to, const void* from)
+__device__ __forceinline__ void copy_async_if(bool there, uint32_t to, const void* from)
 {
-    if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(to), "l"(from) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" :: "r"(to), "l"(from), "n"(BYTES) : "memory");
+    if (BYTES == 16) asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p cp.async.cg.shared.global [%0], [%1], 16;\n\t}" :: "r"(to), "l"(from), "r"((uint32_t)there) : "memory");
+    else asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p cp.async.ca.shared.global [%0], [%1], %3;\n\t}" :: "r"(to), "l"(from), "r"((uint32_t)there), "n"(BYTES) : "memory");
 }
 template <int LEFT>
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_group %0;" :: "n"(LEFT) : "memory"); }
@@ -158,23 +158,17 @@ struct W4Stream {
     {
         w = (const char*)a.qw + unit * 1024 + lane * 16;
         sc = (const char*)a.sc + (unit * 8 + (lane >> 2)) * 4 * GROUPS;
-        if (a.zp) zp = (const char*)a.zp + unit * 16 * GROUPS + ((lane >> 2) * 2 * GROUPS & ~3);
+        zp = (const char*)a.zp + unit * 16 * GROUPS + ((lane >> 2) * 2 * GROUPS & ~3);
     }
-    // asks for the next unit, into the oldest one's place; without one too: the copies are counted
+    // Asks for the next unit, into the oldest one's place; without one too: the copies are counted.  (Predicates, not branches: a branch that the compiler
+    // cannot prove uniform costs three instructions of its own.)
     __device__ __forceinline__ void ask(bool there, bool zeros)
     {
-        if (there)
-        {
-            copy_async<16>(place + at_w, w);
-            copy_async<16>(place + at_w + 512, w + 512);
-            if (scales)
-            {
-                copy_async<4 * GROUPS>(place + at_sc, sc);
-                if (zeros) copy_async<GROUPS == 4 ? 8 : 4>(place + (at_zp & ~3), zp);
-            }
-            w += STEP * 1024; sc += STEP * 32 * GROUPS;
-            if (zeros) zp += STEP * 16 * GROUPS;
-        }
+        copy_async_if<16>(there, place + at_w, w);
+        copy_async_if<16>(there, place + at_w + 512, w + 512);
+        copy_async_if<4 * GROUPS>(there && scales, place + at_sc, sc);
+        if (zeros) copy_async_if<GROUPS == 4 ? 8 : 4>(there && scales, place + (at_zp & ~3), zp);
+        w += STEP * 1024; sc += STEP * 32 * GROUPS; zp += STEP * 16 * GROUPS;
         copies_end();
         place = place == last ? last - (kDepth - 1) * kStage : place + kStage;
     }
