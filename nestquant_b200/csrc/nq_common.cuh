@@ -36,6 +36,8 @@ inline int check_launch(const char* what)
 #ifdef __CUDACC__
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// the same from kernels whose CTAs are one per few rows: only where all of them are there at once (waiting CTAs of a successor take the places of CTAs to come)
+__device__ __forceinline__ void early_signal() { if (gridDim.x <= 592) launch_dependents(); }
 // launch of a kernel that does so; check_launch follows
 template <class... P, class... A>
 inline void launch_dependent(void (*kernel)(P...), dim3 grid, dim3 block, size_t shared, cudaStream_t stream, A... args)

@@ -182,6 +182,8 @@ __device__ __forceinline__ float pick_weight(const Route& a, bool any, float l, 
 template <class L, int PER>
 __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(Route a)
 {
+    early_signal();
+    grid_dependency_wait();
     const int lane = threadIdx.x & 31, t = blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
     if (t >= a.T) return;                                  // warp-uniform
     const L* row = (const L*)a.logits + (size_t)t * a.row_stride;
@@ -303,6 +305,8 @@ struct RouteBwd {
 template <class L, int PER>
 __global__ void __launch_bounds__(32 * kRouteWarps) route_bwd_kernel(RouteBwd a)
 {
+    early_signal();
+    grid_dependency_wait();
     const int lane = threadIdx.x & 31, t = blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
     if (t >= a.T) return;                                  // warp-uniform
     const L* row = (const L*)a.logits + (size_t)t * a.row_stride;
@@ -374,7 +378,7 @@ struct RouteLaunch {
     static void go(Route a, cudaStream_t st)
     {
         a.vec = run_aligned<L, PER>(a.logits, a.row_stride);
-        route_kernel<L, PER><<<(a.T + kRouteWarps - 1) / kRouteWarps, 32 * kRouteWarps, 0, st>>>(a);
+        launch_dependent(route_kernel<L, PER>, dim3((a.T + kRouteWarps - 1) / kRouteWarps), dim3(32 * kRouteWarps), 0, st, a);
     }
 };
 template <class L, int PER>
@@ -382,7 +386,7 @@ struct RouteBwdLaunch {
     static void go(RouteBwd a, cudaStream_t st)
     {
         a.vec = run_aligned<L, PER>(a.logits, a.row_stride) && run_aligned<L, PER>(a.dlogits, a.E);
-        route_bwd_kernel<L, PER><<<(a.T + kRouteWarps - 1) / kRouteWarps, 32 * kRouteWarps, 0, st>>>(a);
+        launch_dependent(route_bwd_kernel<L, PER>, dim3((a.T + kRouteWarps - 1) / kRouteWarps), dim3(32 * kRouteWarps), 0, st, a);
     }
 };
 

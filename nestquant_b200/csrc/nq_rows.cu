@@ -38,6 +38,8 @@ __device__ __forceinline__ void piece_of(size_t i, unsigned pieces, size_t& t, u
 template <class V>
 __global__ void __launch_bounds__(kRowsThreads) dispatch_kernel(Rows a)
 {
+    early_signal();
+    grid_dependency_wait();
     const size_t i = (size_t)blockIdx.x * kRowsThreads + threadIdx.x;
     size_t t;
     unsigned v;
@@ -117,6 +119,8 @@ struct Piece {
 template <class S, class D, int N, bool WEIGHTED>
 __global__ void __launch_bounds__(kRowsThreads) sum_kernel(Rows a)
 {
+    early_signal();
+    grid_dependency_wait();
     const size_t i = (size_t)blockIdx.x * kRowsThreads + threadIdx.x;
     size_t t;
     unsigned v;
@@ -157,6 +161,8 @@ struct CombineBwd {
 template <class Y, class O, int N>
 __global__ void __launch_bounds__(kRowsThreads) combine_bwd_kernel(CombineBwd a)
 {
+    early_signal();
+    grid_dependency_wait();
     __shared__ float s_dot[kRowsThreads / 32][kPicks];
     const int per = 32 * a.warps, slot = threadIdx.x / per, r = threadIdx.x % per, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const size_t t = (size_t)blockIdx.x * (kRowsThreads / per) + slot;
@@ -251,10 +257,10 @@ int sum_rows(Rows a, cudaStream_t st, const char* what)
     a.pieces = a.H / n;
     unsigned grid;
     if (int e = row_grid(a.T, a.pieces, &grid, what)) return e;
-    if (n == 8) { if constexpr (sizeof(S) == 2) sum_kernel<S, D, 8, WEIGHTED><<<grid, kRowsThreads, 0, st>>>(a); }
-    else if (n == 4) sum_kernel<S, D, 4, WEIGHTED><<<grid, kRowsThreads, 0, st>>>(a);
-    else if (n == 2) sum_kernel<S, D, 2, WEIGHTED><<<grid, kRowsThreads, 0, st>>>(a);
-    else sum_kernel<S, D, 1, WEIGHTED><<<grid, kRowsThreads, 0, st>>>(a);
+    if (n == 8) { if constexpr (sizeof(S) == 2) launch_dependent(sum_kernel<S, D, 8, WEIGHTED>, dim3(grid), dim3(kRowsThreads), 0, st, a); }
+    else if (n == 4) launch_dependent(sum_kernel<S, D, 4, WEIGHTED>, dim3(grid), dim3(kRowsThreads), 0, st, a);
+    else if (n == 2) launch_dependent(sum_kernel<S, D, 2, WEIGHTED>, dim3(grid), dim3(kRowsThreads), 0, st, a);
+    else launch_dependent(sum_kernel<S, D, 1, WEIGHTED>, dim3(grid), dim3(kRowsThreads), 0, st, a);
     return check_launch(what);
 }
 
@@ -268,10 +274,10 @@ int combine_bwd(CombineBwd a, cudaStream_t st)
     a.warps = 1;
     while (a.warps < 8 && 32 * a.warps < a.pieces && (long long)a.T * a.warps < 9472) a.warps *= 2;
     const int tokens = kRowsThreads / (32 * a.warps), grid = (a.T - 1) / tokens + 1;
-    if (n == 8) { if constexpr (sizeof(Y) == 2) combine_bwd_kernel<Y, O, 8><<<grid, kRowsThreads, 0, st>>>(a); }
-    else if (n == 4) combine_bwd_kernel<Y, O, 4><<<grid, kRowsThreads, 0, st>>>(a);
-    else if (n == 2) combine_bwd_kernel<Y, O, 2><<<grid, kRowsThreads, 0, st>>>(a);
-    else combine_bwd_kernel<Y, O, 1><<<grid, kRowsThreads, 0, st>>>(a);
+    if (n == 8) { if constexpr (sizeof(Y) == 2) launch_dependent(combine_bwd_kernel<Y, O, 8>, dim3(grid), dim3(kRowsThreads), 0, st, a); }
+    else if (n == 4) launch_dependent(combine_bwd_kernel<Y, O, 4>, dim3(grid), dim3(kRowsThreads), 0, st, a);
+    else if (n == 2) launch_dependent(combine_bwd_kernel<Y, O, 2>, dim3(grid), dim3(kRowsThreads), 0, st, a);
+    else launch_dependent(combine_bwd_kernel<Y, O, 1>, dim3(grid), dim3(kRowsThreads), 0, st, a);
     return check_launch("nq_combine_bwd");
 }
 
@@ -298,10 +304,10 @@ int nq_dispatch(const void* x, int type, long long row_stride, const int32_t* po
     unsigned grid;
     if (int e = nq::row_grid(T, a.pieces, &grid, "nq_dispatch")) return e;
     cudaStream_t st = (cudaStream_t)stream;
-    if (piece == 16) nq::dispatch_kernel<uint4><<<grid, nq::kRowsThreads, 0, st>>>(a);
-    else if (piece == 8) nq::dispatch_kernel<uint2><<<grid, nq::kRowsThreads, 0, st>>>(a);
-    else if (piece == 4) nq::dispatch_kernel<uint32_t><<<grid, nq::kRowsThreads, 0, st>>>(a);
-    else nq::dispatch_kernel<uint16_t><<<grid, nq::kRowsThreads, 0, st>>>(a);
+    if (piece == 16) nq::launch_dependent(nq::dispatch_kernel<uint4>, dim3(grid), dim3(nq::kRowsThreads), 0, st, a);
+    else if (piece == 8) nq::launch_dependent(nq::dispatch_kernel<uint2>, dim3(grid), dim3(nq::kRowsThreads), 0, st, a);
+    else if (piece == 4) nq::launch_dependent(nq::dispatch_kernel<uint32_t>, dim3(grid), dim3(nq::kRowsThreads), 0, st, a);
+    else nq::launch_dependent(nq::dispatch_kernel<uint16_t>, dim3(grid), dim3(nq::kRowsThreads), 0, st, a);
     return nq::check_launch("nq_dispatch");
 }
 
