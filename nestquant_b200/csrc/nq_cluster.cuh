@@ -1,12 +1,37 @@
 // CTAs of a cluster: barrier and distributed shared memory.
 #pragma once
+#include <cuda_runtime.h>
 #include <stdint.h>
+
+#include <atomic>
 
 namespace nq {
 
-// every thread of every CTA of the cluster arrives and waits
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// every thread of every CTA of the cluster arrives and waits, warp by warp
+__device__ __forceinline__ void cluster_arrive()
+{
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait()
+{
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// clusters of ck CTAs of a kernel that the device runs at a time (cfg: its block, shared memory and, as first attribute, cluster size); asked once per
+// kernel, size and device
+template <auto* KERNEL>
+int active_clusters(int ck, int device, cudaLaunchConfig_t& cfg)
+{
+    static std::atomic<int> known[16][4];
+    std::atomic<int>* const at = device < 16 && ck <= 8 ? &known[device][ck == 1 ? 0 : ck == 2 ? 1 : ck == 4 ? 2 : 3] : nullptr;
+    int n = at ? at->load(std::memory_order_relaxed) : 0;
+    if (n) return n;
+    cfg.gridDim = dim3(ck);
+    if (cudaOccupancyMaxActiveClusters(&n, KERNEL, &cfg) != cudaSuccess || n < 1) { cudaGetLastError(); n = 1; }
+    if (at) at->store(n, std::memory_order_relaxed);
+    return n;
+}
 __device__ __forceinline__ uint32_t cluster_address(uint32_t address, int rank)
 {
     uint32_t there;

@@ -1,6 +1,4 @@
 // Products with 4-bit weights (nq_w4.cuh): the layout of the planes, and the kernel for calls of few rows.
-#include <atomic>
-
 #include "nq_tc.cuh"
 #include "nq_w4.cuh"
 
@@ -272,21 +270,6 @@ int w4_chunks(int K) { return (K - 1) / 128 + 1; }
 // bytes between rows of x in shared memory: 64 off a multiple of 128, so that two rows of a fragment share the banks
 int w4_pitch(int C, int ck) { return ((C + ck - 1) / ck) * 256 + 64; }
 
-// clusters of ck CTAs that the device runs at a time, one CTA per SM
-template <auto* KERNEL>
-int w4_clusters(int ck, int sms, int device, cudaLaunchConfig_t& cfg)
-{
-    static std::atomic<int> known[16][4];
-    if (ck == 1) return sms;
-    std::atomic<int>* const at = device < 16 ? &known[device][ck == 2 ? 0 : ck == 4 ? 1 : 2] : nullptr;
-    int n = at ? at->load(std::memory_order_relaxed) : 0;
-    if (n) return n;
-    cfg.gridDim = dim3(ck);
-    if (cudaOccupancyMaxActiveClusters(&n, KERNEL, &cfg) != cudaSuccess || n < 1) { cudaGetLastError(); n = 1; }
-    if (at) at->store(n, std::memory_order_relaxed);
-    return n;
-}
-
 // How a matrix is cut: CTAs of a cluster and warps of a CTA that share a strip, both powers of two.  The device takes ceil(blocks / clusters) rounds; a round
 // costs a warp its units and what comes per item (measured: sums and barriers as much as a unit and a half, over a cluster three).
 // calls for the other kernel
@@ -305,7 +288,7 @@ bool w4_cut(W4& a, int rows, int device, cudaLaunchConfig_t& cfg, long long& clu
         cudaLaunchAttribute& cluster = cfg.attrs[0];
         cluster.val.clusterDim.x = ck;
         cfg.dynamicSmemBytes = Plan::kPlanes + Plan::kParts + (size_t)rows * w4_pitch(a.C, ck);
-        const int there = w4_clusters<w4_kernel<X, SC, GROUPS, TILES>>(ck, a.sms, device, cfg);
+        const int there = ck == 1 ? a.sms : active_clusters<w4_kernel<X, SC, GROUPS, TILES>>(ck, device, cfg);
         for (int log_wk = 0; log_wk <= 4 && ck << log_wk <= a.C; ++log_wk)
         {
             const int blocks = (a.S - 1) / (kW4Warps >> log_wk) + 1, units = ((a.C - 1) >> (log_ck + log_wk)) + 1;

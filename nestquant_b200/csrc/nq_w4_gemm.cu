@@ -497,18 +497,26 @@ int wg_launch(Wg g, int device, cudaStream_t st)
     a.blocks = (a.S - 1) / 8 + 1;
     const long long most = (long long)a.blocks * (a.start ? a.rows / TOKENS + (a.E < a.rows ? a.E : a.rows) : (a.rows - 1) / TOKENS + 1);
     NQ_REQUIRE(most <= 0x7fffffff / a.C, "nq_w4_matmul: %d rows are too many", a.rows);
-    // columns are split while that leaves a cluster for every item
-    g.log_ck = 0;
-    while (!a.start && g.log_ck < 3 && a.C >> (g.log_ck + 1) >= 2 && most << (g.log_ck + 1) <= a.sms) ++g.log_ck;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 1 << g.log_ck; attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr; cfg.numAttrs = 2;
+    cfg.attrs = attr; cfg.numAttrs = 1;
+    cfg.blockDim = dim3(Plan::kThreads); cfg.dynamicSmemBytes = Plan::kSmem; cfg.stream = st;
+    // columns are split while every item still has a cluster at once
+    g.log_ck = 0;
+    for (int log_ck = 1; !a.start && log_ck <= 3 && a.C >> log_ck >= 2 && most << log_ck <= a.sms; ++log_ck)
+    {
+        attr[0].val.clusterDim.x = 1 << log_ck;
+        if (most > active_clusters<w4_gemm_kernel<X, SC, GROUPS, TOKENS>>(1 << log_ck, device, cfg)) break;
+        g.log_ck = log_ck;
+    }
+    attr[0].val.clusterDim.x = 1 << g.log_ck;
+    cfg.numAttrs = 2;
     const long long clusters = g.log_ck ? most : most < a.sms ? most : a.sms;
-    cfg.gridDim = dim3((unsigned)(clusters << g.log_ck)); cfg.blockDim = dim3(Plan::kThreads); cfg.dynamicSmemBytes = Plan::kSmem; cfg.stream = st;
+    cfg.gridDim = dim3((unsigned)(clusters << g.log_ck));
     cudaLaunchKernelEx(&cfg, kernel, map, g);
     return check_launch("nq_w4_matmul");
 }
