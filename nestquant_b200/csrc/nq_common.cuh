@@ -36,7 +36,8 @@ inline int check_launch(const char* what)
 #ifdef __CUDACC__
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-// the same from kernels whose CTAs are one per few rows: only where all of them are there at once (waiting CTAs of a successor take the places of CTAs to come)
+// the same from kernels whose CTAs are one per few rows: only where all of them are there at once (waiting CTAs of a successor take
+// the places of CTAs to come).  route, sort, dispatch and combine of 16 tokens, captured: 11.2 us without early launches, 9.6 with them
 __device__ __forceinline__ void early_signal() { if (gridDim.x <= 592) launch_dependents(); }
 // launch of a kernel that does so; check_launch follows
 template <class... P, class... A>

@@ -15,7 +15,8 @@
 // further apart than 6e-7 + 3e-7 |score| are in the right order, and so are equal logits with equal biases; a row with any other
 // neighbours among its first topk + 1 is put in order again in 64 bits (one row of a thousand, with 256 experts).
 //
-// A warp per row; lane i holds the experts [i PER, (i + 1) PER), so that the lowest lane that has the largest key also has the lowest id.
+// A warp per row; lane i holds the experts [i PER, (i + 1) PER), so that the lowest lane that has the largest key also has the lowest id.  The logits are read once
+// (floor of 16,384 rows of 256: 2.8 us, and as much for the gradient's zeros); bound by instructions: 16 us with a bias, 11 without, gradient 8.6.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -216,8 +217,8 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(Route a)
         key[i] = ok ? float_key(s) : 0u;
     }
     // Pick j to lane j, and behind a biased choice the one that follows it.  No key below the picks-th largest of the lanes' largest keys is among the picks
-    // largest, so the few that are not go to the lanes, one each, and count how many are in front of them.  (Taking the largest away pick by pick cost
-    // 48 instructions a pick: 16,384 rows of 256 16.5 us.)
+    // largest, so the few that are not go to the lanes, one each, and count how many are in front of them.  (Taking the largest away pick by pick takes
+    // 48 instructions a pick: 16,384 rows of 256 16.5 us without a bias instead of 11.)
     __shared__ uint2 s_found[kRouteWarps][2][34];          // {key, expert}: as found, in order
     uint2 (&found)[2][34] = s_found[threadIdx.x >> 5];
     unsigned my_key = 0, next_key = 0;

@@ -115,6 +115,13 @@ __device__ __forceinline__ void strip_product(STREAM& planes, int units, bool ze
         for (int i = 0; i < 4; ++i) acc[n][i] = sum[n][i];
 }
 
+// For calls of up to 16 rows: bound by HBM by intent, by the instructions that unpack the weights in practice.  A unit costs a warp 152 instructions (32 masks, 8 shifts,
+// 32 half-pair additions, 8 MMAs; 57 of them on the half-rate integer pipe, 20 for a share of its item's sums), four warps of a scheduler issue in two thirds of the
+// clocks.  us, captured, one launch after the other, 1 / 8 / 16 rows of 4,096 x 6,144 (floor 2.0): 5.7 / 7.6 / 9.5; one row of 32,768 x 8,192 31 (4.5 TB/s;
+// floor 21), of 16 x 128 2.4.  What made the difference, one row of 32,768 x 8,192: units asked for ahead into registers 57 (their loads shared the few scoreboards);
+// through shared memory, a CTA per block of strips 55; one CTA per SM with units asked for across items 43; cuts in shifts instead of 64-bit divisions 39; masks as one
+// instruction each 34; cuts by rounds 32; predicates instead of branches 31.  32 warps of 64 registers: 35.
+//
 // One CTA per SM, in clusters of `ck` that split the matrix into ranges of columns, each taking a run of consecutive items.  A block has ws = 16 / wk strips, wk
 // warps for each: part p = rank wk + warp % wk of parts = ck wk multiplies the units [p C / parts, (p + 1) C / parts) of its strip with up to 8 TILES rows
 // of x, which stay in shared memory as long as the rows are the same.  Units are asked for across the borders of items, so that memory does not
@@ -271,8 +278,10 @@ int w4_chunks(int K) { return (K - 1) / 128 + 1; }
 int w4_pitch(int C, int ck) { return ((C + ck - 1) / ck) * 256 + 64; }
 
 // How a matrix is cut: CTAs of a cluster and warps of a CTA that share a strip, both powers of two.  The device takes ceil(blocks / clusters) rounds; a round
-// costs a warp its units and what comes per item (measured: sums and barriers as much as a unit and a half, over a cluster three).
-// calls for the other kernel
+// costs a warp its units and what comes per item (sums and barriers: as much as a unit and a half, over a cluster three).  Rows of x weigh in so that 8 rows of
+// 6,144 columns, 98 KB for each CTA of its own, are shared by two CTAs: 7.6 us instead of 8.2.
+// Calls for the other kernel.  us, this kernel / that one, 4,096 x 6,144: 16 rows 9.5 / 11.3, 32 rows (four tiles here) 15.4 / 10.8; 6,144 x 2,048 in groups of 64:
+// 7.2 / 9.8, 11.4 / 9.8; 16,384 x 8,192, 16 rows: 27 / 37.
 bool w4_many_rows(int rows, int E, const int* start) { return (start ? rows / E : rows) > 16; }
 
 template <class X, class SC, int GROUPS, int TILES>

@@ -7,6 +7,11 @@
 //   TMA        (one warp) the tokens' tiles [TOKENS x 64], two per chunk of 128 columns
 //   MMAs       (one warp) an elected lane issues tcgen05.mma, 128 x TOKENS x 16 a step, into one of two accumulators per group of columns: an accumulator
 //              holds one group's sum only, so that the scale is applied in 32 bits and nothing is rounded before the result
+// Bound by the tensor pipe by intent; in practice by the tokens' tiles from L2 (each CTA reads its own: 37 bytes per clock and SM at 512 rows) and by the issue slots that
+// weights and sums share with the MMAs.  us, rows of 4,096 x 6,144 in groups of 128 (tensor floor): 32 10.8, 64 12.2, 128 14.3 (3.9), 512 28.5 (15.7), 2,048 105
+// (62.8) = 0.98 PFLOP/s; in groups of 32, 512 rows, 65: four times the sums.  What made the difference at 512 rows: one row block of 32 per pass of the other kernel
+// 156; this kernel with eight warps of 128 tokens' sums and the MMAs one by one 35; registers by role and two sums an instruction 30.  Passes of up to 64 rows: an MMA of
+// 16 columns takes ~56 clocks however few tokens it has, and sixteen warps decode.
 // Columns of an item may be split over a cluster; each CTA then adds up a share of the tokens, the others' sums come through distributed shared memory.
 // Every mbarrier wait is bounded (nq_tc.cuh): on time-out the CTA raises status[0], waits for its loads and MMAs in flight and ends.
 #include "nq_tc.cuh"
