@@ -342,7 +342,7 @@ int nq_combine_bwd(const void* dout, int out_type, const void* y, int type, cons
 
 /* Matrices of 4-bit weights: (q[n][k] - z[n][k / group]) * s[n][k / group], group 32, 64 or 128, a divisor of K.
  *   nq_w4_units   number of units (16 rows x 128 columns) of E matrices N x K
- *   nq_w4_layout  q uint8 [E][N][K / 2] (two columns a byte, the even one in the low half), scales [E][N][K / group] of any 16-bit type, zeros uint8
+ *   nq_w4_layout  q uint8 [E][N][K / 2] (two columns a byte, the even one in the low half; on an even address), scales [E][N][K / group] of any 16-bit type, zeros uint8
  *                 [E][N][K / group] (0 to 15) or NULL (8) -> planes qw [units][1024] bytes, sc [units][16 * 128 / group] 16-bit, zp likewise bytes (NULL
  *                 without zeros), in the order of nq_w4.cu
  *   nq_w4_matmul  out[r] = W x[r] for x [rows][x_stride >= K] of `type` (NQ_F16 or NQ_BF16; rows start on 16 bytes), out [rows][out_stride >= N] of type

@@ -285,7 +285,9 @@ W4Ptr w4_planes(const Tensor& q_, const Tensor& scales_, const c10::optional<Ten
     int64_t units;
     check(nq_w4_units((int)w->E, (int)w->N, (int)w->K, &units), "W4");
     const c10::cuda::CUDAGuard guard(q_.device());
-    const Tensor q = q_.contiguous(), scales = scales_.contiguous(), zeros = zeros_ ? zeros_->contiguous() : Tensor();
+    Tensor q = q_.contiguous();
+    if (reinterpret_cast<uintptr_t>(q.data_ptr()) % 2) q = q.clone();       // (read two bytes at a time)
+    const Tensor scales = scales_.contiguous(), zeros = zeros_ ? zeros_->contiguous() : Tensor();
     const int64_t per = 16 * (128 / w->group);
     w->qw = at::empty({units * 1024}, q.options());
     w->sc = at::empty({units * per}, scales.options());

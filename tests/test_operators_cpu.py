@@ -39,7 +39,7 @@ MATMUL = dict(x=P, type=NQ_F16, x_stride=256, qw=P, sc=P, sc_type=NQ_F16, zp=P, 
     ("nq_dispatch_bwd", DISPATCH_BWD, [dict(type=5), dict(T=-1), dict(topk=0), dict(H=0), dict(dxs=None), dict(pos=None), dict(live=None), dict(dx=None)]),
     ("nq_combine", COMBINE, [dict(type=7), dict(rw_type=9), dict(out_type=NQ_BF16), dict(T=-1), dict(topk=0), dict(H=0), dict(y=None), dict(rw=None), dict(out=None)]),
     ("nq_combine_bwd", COMBINE_BWD, [dict(type=7), dict(rw_type=9), dict(out_type=NQ_BF16), dict(T=-1), dict(H=0), dict(dout=None), dict(y=None), dict(rw=None), dict(pos=None)]),
-    ("nq_w4_layout", LAYOUT, [dict(group=16), dict(group=256), dict(K=96, group=64), dict(K=0), dict(N=0), dict(E=0), dict(q=None), dict(zp=None), dict(zeros=None), dict(qw=P + 8)]),
+    ("nq_w4_layout", LAYOUT, [dict(group=16), dict(group=256), dict(K=96, group=64), dict(K=0), dict(N=0), dict(E=0), dict(q=None), dict(zp=None), dict(zeros=None), dict(qw=P + 8), dict(q=P + 1)]),
     ("nq_w4_matmul", MATMUL, [dict(type=NQ_F32), dict(sc_type=NQ_F32), dict(out_type=NQ_BF16), dict(group=48), dict(K=320, group=128), dict(rows=-1), dict(start=None), dict(x_stride=255),
                               dict(x_stride=260), dict(out_stride=63), dict(x=P + 8), dict(x=None), dict(qw=None), dict(sc=None), dict(out=None), dict(status=None), dict(E=0), dict(E=1025)]),
 ] for o in overs], ids=lambda v: v if isinstance(v, str) else ",".join(f"{a}={b}" for a, b in v.items()) if len(v) < 4 else "")

@@ -110,6 +110,11 @@ def test_strided_and_unaligned_rows():
     for x in (buf[:9, :128], buf[:9, 8:136], buf[:9, 3:131], buf[::5, 16:144], buf.t()[:20, :128] if buf.shape[0] >= 128 else buf[:, :128], buf[:1, :128].expand(5, 128), buf[4:5, 1:129]):
         check(w(x), x, W, 128)
     assert w(buf[:0, :128]).shape == (0, 40)
+    odd = torch.empty(q.numel() + 1, dtype=torch.uint8, device="cuda")[1:].view(q.shape).copy_(q)      # weights off two bytes, strided scales
+    wide = torch.empty(40, 6, dtype=s.dtype, device="cuda")
+    wide[:, ::3] = s
+    x = buf[:9, :128]
+    assert torch.equal(w4.W4(odd, wide[:, ::3], z.t().contiguous().t())(x), w(x))
 
 
 def test_values_that_are_not_finite_stay_in_their_rows():
