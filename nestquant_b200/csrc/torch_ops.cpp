@@ -127,14 +127,13 @@ struct Order : torch::CustomClassHolder {
     int64_t T, topk, E;
     Tensor buf;
     int64_t P() const { return T * topk; }
-    Tensor start() const { return buf.narrow(0, 0, E + 1); }
-    Tensor flat() const { return buf.narrow(0, E + 2, P()); }
-    Tensor pos() const { return flat().view({T, topk}); }
+    Tensor start() const { return buf.as_strided({E + 1}, {1}, 0); }
+    Tensor pos() const { return buf.as_strided({T, topk}, {topk, 1}, E + 2); }
     Tensor token() const
     {
         const c10::cuda::CUDAGuard guard(buf.device());
         const Tensor picks = at::arange(P(), buf.options());
-        return at::empty_like(picks).scatter_(0, flat().to(at::kLong), at::floor_divide(picks, topk));
+        return at::empty_like(picks).scatter_(0, pos().flatten().to(at::kLong), at::floor_divide(picks, topk));
     }
     Tensor expert() const
     {
