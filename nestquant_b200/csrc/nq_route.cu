@@ -10,13 +10,15 @@
 //             sigmoid as it is      dl_j = c g_j s_j (1 - s_j);   softmax as it is: dl_e = c p_e (g_e - sum_i g_i p_i), g_e = 0 elsewhere.
 //
 // With a bias the order has to be that of the real numbers, not of their roundings to 32 bits, whose ties would depend on how the
-// exponential is computed.  |fp32 score - score| <= 1.8e-7 + 6e-8 |score|: expf has 2 ulp, which the slope s (1 - s) <= 1/4 makes
-// 6e-8; the sum and the quotient round once each, 6e-8 s; the bias adds 6e-8 |score|.  Two neighbours in the sorted list that are
+// exponential is computed.  |fp32 score - score| <= 2.7e-7 + 6e-8 |score| with the hardware's exponential and reciprocal: the argument's rounding is off by
+// 2^-24 |l|, the power of two by 2^-22 of its value, which the slope s (1 - s) <= min(1/4, e^-|l|) makes 2.2e-8 and 6e-8; the sum rounds by 6e-8 s and
+// the reciprocal is off by 1.2e-7 s; the bias adds 6e-8 |score|.  Two neighbours in the sorted list that are
 // further apart than 6e-7 + 3e-7 |score| are in the right order, and so are equal logits with equal biases; a row with any other
 // neighbours among its first topk + 1 is put in order again in 64 bits (one row of a thousand, with 256 experts).
 //
 // A warp per row; lane i holds the experts [i PER, (i + 1) PER), so that the lowest lane that has the largest key also has the lowest id.  The logits are read once
-// (floor of 16,384 rows of 256: 2.8 us, and as much for the gradient's zeros); bound by instructions: 16 us with a bias, 11 without, gradient 8.6.
+// (floor of 16,384 rows of 256: 2.8 us, and as much for the gradient's zeros); bound by instructions: 14 us with a bias (16 with
+// exponential and division as the weights have them), 11 without, gradient 8.4.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -39,6 +41,8 @@ __device__ __forceinline__ bool eligible(float f) { return f > -INFINITY; }     
 __device__ __forceinline__ float in_doubt_below(float score) { return 6e-7f + 3e-7f * fabsf(score); }
 __device__ __forceinline__ double exact_score(float l, float b) { return 1.0 / (1.0 + exp(-(double)l)) + (double)b; }
 __device__ __forceinline__ float sigmoid(float l) { return 1.f / (1.f + expf(-l)); }
+// for the order alone (see above)
+__device__ __forceinline__ float quick_sigmoid(float l) { return __fdividef(1.f, 1.f + __expf(-l)); }
 __device__ __forceinline__ float warp_sum(float v)
 {
 #pragma unroll
@@ -164,7 +168,7 @@ __device__ __noinline__ void choose_one_by_one(const unsigned (&keys)[PER], int 
 struct Route {
     const void* logits; const float* bias; int64_t* sel; void* rw;
     long long row_stride;
-    int T, E, topk, softmax, renorm, rw_type, vec;
+    int T, E, topk, softmax, renorm, rw_type, vec, vec_bias;
     float scale;
 };
 
@@ -202,20 +206,16 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(Route a)
         denominator = warp_sum(s);
     }
     unsigned key[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
+    if (a.bias)
     {
-        const int e = lane * PER + i;
-        float s = v[i];
-        bool ok = eligible(s);
-        if (a.bias)
-        {
-            const float b = e < a.E ? a.bias[e] : -INFINITY;
-            ok = ok && eligible(b);
-            s = sigmoid(s) + b;
-        }
-        key[i] = ok ? float_key(s) : 0u;
+        float b[PER];
+        load_run<float, PER>(a.bias, lane * PER, a.E, a.vec_bias, b);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) key[i] = eligible(v[i]) && eligible(b[i]) ? float_key(quick_sigmoid(v[i]) + b[i]) : 0u;
     }
+    else
+#pragma unroll
+        for (int i = 0; i < PER; ++i) key[i] = eligible(v[i]) ? float_key(v[i]) : 0u;
     // Pick j to lane j, and behind a biased choice the one that follows it.  No key below the picks-th largest of the lanes' largest keys is among the picks
     // largest, so the few that are not go to the lanes, one each, and count how many are in front of them.  (Taking the largest away pick by pick takes
     // 48 instructions a pick: 16,384 rows of 256 16.5 us without a bias instead of 11.)
@@ -379,6 +379,7 @@ struct RouteLaunch {
     static void go(Route a, cudaStream_t st)
     {
         a.vec = run_aligned<L, PER>(a.logits, a.row_stride);
+        a.vec_bias = run_aligned<float, PER>(a.bias, PER);
         launch_dependent(route_kernel<L, PER>, dim3((a.T + kRouteWarps - 1) / kRouteWarps), dim3(32 * kRouteWarps), 0, st, a);
     }
 };
@@ -410,7 +411,7 @@ int nq_route(const void* logits, int type, long long row_stride, const float* bi
     NQ_REQUIRE(!(score == 1 && bias), "nq_route: a bias goes with sigmoid scores");
     if (T == 0) return NQ_OK;
     NQ_REQUIRE(logits && sel && rw, "nq_route: null pointer");
-    nq::by_width<nq::RouteLaunch>(type, E, nq::Route{logits, bias, sel, rw, row_stride, T, E, topk, score, renorm != 0, rw_type, 0, scale}, (cudaStream_t)stream);
+    nq::by_width<nq::RouteLaunch>(type, E, nq::Route{logits, bias, sel, rw, row_stride, T, E, topk, score, renorm != 0, rw_type, 0, 0, scale}, (cudaStream_t)stream);
     return nq::check_launch("nq_route");
 }
 
