@@ -100,7 +100,7 @@ __device__ __forceinline__ void fma_two(uint64_t& sum, uint64_t s, uint32_t x, u
 }
 
 // (mbar_wait_warp with its slow part in line: a call would take the registers that the sums are in)
-__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, PfWaits* waits)
+__device__ __forceinline__ bool wait_bar_slow(uint32_t bar, uint32_t parity, PfWaits* waits)
 {
     unsigned long long t0 = 0, t;
     while (!__all_sync(0xffffffffu, mbar_poll(bar, parity)))
@@ -111,6 +111,11 @@ __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, PfWaits*
         else if (__any_sync(0xffffffffu, t - t0 > waits->limit_ns)) { waits->aborted = 1; return false; }
     }
     return true;
+}
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, PfWaits* waits)
+{
+    if (__builtin_expect(__all_sync(0xffffffffu, mbar_poll(bar, parity)), 1)) return true;
+    return wait_bar_slow(bar, parity, waits);
 }
 // (likewise mbar_wait_own)
 __device__ __forceinline__ void wait_own(uint32_t bar, uint32_t parity)
@@ -421,16 +426,22 @@ __global__ void __launch_bounds__((WgPlan<GROUPS, TOKENS>::kThreads), 1) w4_gemm
         bool ok = true;
         for (int u = (i1 - i0) * (c1 - c0); u > 0 && ok; --u)
         {
-            ok = wait_bar(saddr(&sh.full_a[stage.s]), stage.parity, &sh.waits) && wait_bar(saddr(&sh.full_b[stage.s]), stage.parity, &sh.waits);
+            // weights, tokens and an accumulator: three polls, one vote (a wait each, all of them complete, took 450 of 980 clocks a chunk)
+            uint32_t ready = mbar_poll(saddr(&sh.full_a[stage.s]), stage.parity);
+            ready &= mbar_poll(saddr(&sh.full_b[stage.s]), stage.parity);
+            ready &= mbar_poll(saddr(&sh.sum_empty[acc.s]), acc.parity ^ 1u);
+            if (__builtin_expect(!__all_sync(0xffffffffu, ready), 0))
+                ok = wait_bar_slow(saddr(&sh.full_a[stage.s]), stage.parity, &sh.waits) && wait_bar_slow(saddr(&sh.full_b[stage.s]), stage.parity, &sh.waits) &&
+                     wait_bar_slow(saddr(&sh.sum_empty[acc.s]), acc.parity ^ 1u, &sh.waits);
             const uint32_t w = tmem + 2 * Plan::kSumColumns + stage.s * 64, b_lo = b0 + stage.s * (2 * Plan::kBox >> 4);
             auto group = [&](auto j) {
                 constexpr int kSteps = 8 / GROUPS, kFirst = decltype(j)::value * kSteps;
                 if constexpr (kFirst < 8)
                 {
                     constexpr int kPlace = decltype(j)::value % Plan::kSet;      // in the accumulator
-                    if (kPlace == 0) ok = ok && wait_bar(saddr(&sh.sum_empty[acc.s]), acc.parity ^ 1u, &sh.waits);
+                    if (kPlace == 0 && kFirst) ok = ok && wait_bar(saddr(&sh.sum_empty[acc.s]), acc.parity ^ 1u, &sh.waits);
                     if (!ok) return;
-                    tc_fence_after();
+                    if (kPlace == 0) tc_fence_after();
                     mma_group<kSteps, Plan::kBox, kPlace == Plan::kSet - 1>(tmem + acc.s * Plan::kSumColumns + kPlace * TOKENS, w + kFirst * 8,
                                                                              b_lo + (kFirst >> 2) * (Plan::kBox >> 4) + (kFirst & 3) * 2, b_hi, kDesc, saddr(&sh.sum_full[acc.s]));
                     if (kPlace == Plan::kSet - 1) acc.next();
