@@ -14,6 +14,8 @@
 // 16 columns takes ~56 clocks however few tokens it has, and sixteen warps decode.
 // Columns of an item may be split over a cluster; each CTA then adds up a share of the tokens, the others' sums come through distributed shared memory.
 // Every mbarrier wait is bounded (nq_tc.cuh): on time-out the CTA raises status[0], waits for its loads and MMAs in flight and ends.
+#include <stddef.h>
+
 #include "nq_tc.cuh"
 #include "nq_w4.cuh"
 
@@ -53,20 +55,26 @@ __device__ __forceinline__ void tma_two_boxes(uint32_t dst, uint32_t box, const 
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                  ::"r"(dst + box), "l"(map), "r"(x + 64), "r"(y), "r"(bar) : "memory");
 }
-// The MMAs of a group of STEPS steps of 16 columns and, with COMMIT, the commit to `full`, by one elected lane (one election, few instructions: this warp shares its scheduler
-// with busy ones).  Weights in tensor memory, 8 columns a step; tokens in shared memory, two tiles of 64 columns, BOX bytes apart (the descriptor counts in 16
-// bytes).  The first MMA overwrites the accumulator.
+// The MMAs of a group of STEPS steps of 16 columns, by one elected lane (one election, few instructions: this warp shares its scheduler with busy ones), with FULL the
+// commit to the barrier `full` and with EMPTY that to `empty`.  Weights in tensor memory, 8 columns a step; tokens in shared memory, two tiles of 64 columns, BOX bytes
+// apart (the descriptor counts in 16 bytes).  The first MMA overwrites the accumulator.
 #define NQ_WG_STEP(A, B, P) \
     "add.u32 ta, %1, " A ";\n\tadd.u32 tb, %2, " B ";\n\tmov.b64 db, {tb, %3};\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], [ta], db, %4, " P ";\n\t"
-#define NQ_WG_GROUP(STEPS_TEXT, COMMIT)                                                                                                                       \
+#define NQ_WG_COMMIT(BAR) "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [" BAR "];\n\t"
+#define NQ_WG_GROUP(STEPS_TEXT, COMMITS)                                                                                                                      \
     asm volatile("{\n\t.reg .pred p, q, e;\n\t.reg .b64 db;\n\t.reg .b32 ta, tb;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 p, %4, %4;\n\tsetp.eq.u32 q, %4, %4;\n\t"  \
-                 STEPS_TEXT COMMIT "}"                                                                                                                 \
-                 ::"r"(d), "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(full), "n"(BOX >> 4) : "memory")
-#define NQ_WG_COMMIT "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%5];\n\t"
-#define NQ_WG_EITHER(STEPS_TEXT) do { if (COMMIT) NQ_WG_GROUP(STEPS_TEXT, NQ_WG_COMMIT); else NQ_WG_GROUP(STEPS_TEXT, ""); } while (0)
-template <int STEPS, int BOX, bool COMMIT>
-__device__ __forceinline__ void mma_group(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t full)
+                 STEPS_TEXT COMMITS "}"                                                                                                                \
+                 ::"r"(d), "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(full), "n"(BOX >> 4), "r"(empty) : "memory")
+#define NQ_WG_EITHER(STEPS_TEXT)                                                             \
+    do {                                                                                     \
+        if (FULL && EMPTY) NQ_WG_GROUP(STEPS_TEXT, NQ_WG_COMMIT("%5") NQ_WG_COMMIT("%7"));   \
+        else if (FULL) NQ_WG_GROUP(STEPS_TEXT, NQ_WG_COMMIT("%5"));                          \
+        else NQ_WG_GROUP(STEPS_TEXT, "");                                                    \
+    } while (0)
+template <int STEPS, int BOX, bool FULL, bool EMPTY>
+__device__ __forceinline__ void mma_group(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t full, uint32_t empty)
 {
+    static_assert(FULL || !EMPTY, "a chunk's last group is the last of an accumulator");
     if constexpr (STEPS == 8)
         NQ_WG_EITHER(NQ_WG_STEP("0", "0", "p") NQ_WG_STEP("8", "2", "q") NQ_WG_STEP("16", "4", "q") NQ_WG_STEP("24", "6", "q")
                      NQ_WG_STEP("32", "%6", "q") NQ_WG_STEP("40", "%6+2", "q") NQ_WG_STEP("48", "%6+4", "q") NQ_WG_STEP("56", "%6+6", "q"));
@@ -421,35 +429,51 @@ __global__ void __launch_bounds__((WgPlan<GROUPS, TOKENS>::kThreads), 1) w4_gemm
         constexpr uint32_t kDesc = (1u << 4) | (kType << 7) | (kType << 10) | ((uint32_t)(TOKENS >> 3) << 17) | (8u << 24);      // fp32 sums, both operands K-major, M 128
         const uint64_t desc = smem_desc(saddr(wg_smem), 16, 1024, 2);
         const uint32_t b0 = (uint32_t)desc, b_hi = (uint32_t)(desc >> 32);
-        Ring<kStages> stage;
-        Ring<2> acc;
+        // Stages and accumulators are constants here, so that the addresses are: what this warp issues beside the MMAs paces the kernel
+        const uint32_t bars = saddr(&sh);
+        uint32_t stage_parity = 0, sum_parity = 0;        // (of accumulator a: bit a)
+        int left = (i1 - i0) * (c1 - c0);
         bool ok = true;
-        for (int u = (i1 - i0) * (c1 - c0); u > 0 && ok; --u)
+        auto chunk = [&](auto stage) {
+            constexpr int kS = decltype(stage)::value, kSets = GROUPS / Plan::kSet, kFirstSum = kS * kSets & 1;
+            constexpr int kA = offsetof(WgShared, full_a) + 8 * kS, kB = offsetof(WgShared, full_b) + 8 * kS, kEmpty = offsetof(WgShared, empty) + 8 * kS;
+            if constexpr (kS < kStages)
+            {
+                if (left <= 0) return;
+                // weights, tokens and an accumulator: three polls, one vote (a wait each, all of them complete, took 450 of 980 clocks a chunk)
+                const uint32_t free_parity = ((sum_parity >> kFirstSum) & 1u) ^ 1u;
+                uint32_t ready = mbar_poll(bars + kA, stage_parity);
+                ready &= mbar_poll(bars + kB, stage_parity);
+                ready &= mbar_poll(bars + offsetof(WgShared, sum_empty) + 8 * kFirstSum, free_parity);
+                if (__builtin_expect(!__all_sync(0xffffffffu, ready), 0))
+                    ok = wait_bar_slow(bars + kA, stage_parity, &sh.waits) && wait_bar_slow(bars + kB, stage_parity, &sh.waits) &&
+                         wait_bar_slow(bars + offsetof(WgShared, sum_empty) + 8 * kFirstSum, free_parity, &sh.waits);
+                const uint32_t w = tmem + 2 * Plan::kSumColumns + kS * 64, b_lo = b0 + kS * (2 * Plan::kBox >> 4);
+                auto group = [&](auto j) {
+                    constexpr int kJ = decltype(j)::value, kSteps = 8 / GROUPS, kFirst = kJ * kSteps;
+                    if constexpr (kJ < GROUPS)
+                    {
+                        constexpr int kPlace = kJ % Plan::kSet, kSum = (kS * kSets + kJ / Plan::kSet) & 1;      // in the accumulator, and which
+                        constexpr int kFree = offsetof(WgShared, sum_empty) + 8 * kSum, kFull = offsetof(WgShared, sum_full) + 8 * kSum;
+                        if (kPlace == 0 && kJ) ok = ok && wait_bar(bars + kFree, ((sum_parity >> kSum) & 1u) ^ 1u, &sh.waits);
+                        if (!ok) return;
+                        if (kPlace == 0) tc_fence_after();
+                        mma_group<kSteps, Plan::kBox, kPlace == Plan::kSet - 1, kJ == GROUPS - 1>(
+                            tmem + kSum * Plan::kSumColumns + kPlace * TOKENS, w + kFirst * 8, b_lo + (kFirst >> 2) * (Plan::kBox >> 4) + (kFirst & 3) * 2, b_hi, kDesc,
+                            bars + kFull, bars + kEmpty);
+                        if (kPlace == Plan::kSet - 1) sum_parity ^= 1u << kSum;
+                    }
+                };
+                group(std::integral_constant<int, 0>()); group(std::integral_constant<int, 1>()); group(std::integral_constant<int, 2>()); group(std::integral_constant<int, 3>());
+                left = ok ? left - 1 : 0;
+            }
+        };
+        static_assert(kStages % 2 == 0 && kStages <= 6, "a round of the stages leaves the accumulators where they were");
+        while (left > 0)
         {
-            // weights, tokens and an accumulator: three polls, one vote (a wait each, all of them complete, took 450 of 980 clocks a chunk)
-            uint32_t ready = mbar_poll(saddr(&sh.full_a[stage.s]), stage.parity);
-            ready &= mbar_poll(saddr(&sh.full_b[stage.s]), stage.parity);
-            ready &= mbar_poll(saddr(&sh.sum_empty[acc.s]), acc.parity ^ 1u);
-            if (__builtin_expect(!__all_sync(0xffffffffu, ready), 0))
-                ok = wait_bar_slow(saddr(&sh.full_a[stage.s]), stage.parity, &sh.waits) && wait_bar_slow(saddr(&sh.full_b[stage.s]), stage.parity, &sh.waits) &&
-                     wait_bar_slow(saddr(&sh.sum_empty[acc.s]), acc.parity ^ 1u, &sh.waits);
-            const uint32_t w = tmem + 2 * Plan::kSumColumns + stage.s * 64, b_lo = b0 + stage.s * (2 * Plan::kBox >> 4);
-            auto group = [&](auto j) {
-                constexpr int kSteps = 8 / GROUPS, kFirst = decltype(j)::value * kSteps;
-                if constexpr (kFirst < 8)
-                {
-                    constexpr int kPlace = decltype(j)::value % Plan::kSet;      // in the accumulator
-                    if (kPlace == 0 && kFirst) ok = ok && wait_bar(saddr(&sh.sum_empty[acc.s]), acc.parity ^ 1u, &sh.waits);
-                    if (!ok) return;
-                    if (kPlace == 0) tc_fence_after();
-                    mma_group<kSteps, Plan::kBox, kPlace == Plan::kSet - 1>(tmem + acc.s * Plan::kSumColumns + kPlace * TOKENS, w + kFirst * 8,
-                                                                             b_lo + (kFirst >> 2) * (Plan::kBox >> 4) + (kFirst & 3) * 2, b_hi, kDesc, saddr(&sh.sum_full[acc.s]));
-                    if (kPlace == Plan::kSet - 1) acc.next();
-                }
-            };
-            group(std::integral_constant<int, 0>()); group(std::integral_constant<int, 1>()); group(std::integral_constant<int, 2>()); group(std::integral_constant<int, 3>());
-            if (ok) tc_commit_elect(&sh.empty[stage.s]);
-            stage.next();
+            chunk(std::integral_constant<int, 0>()); chunk(std::integral_constant<int, 1>()); chunk(std::integral_constant<int, 2>());
+            chunk(std::integral_constant<int, 3>()); chunk(std::integral_constant<int, 4>()); chunk(std::integral_constant<int, 5>());
+            stage_parity ^= 1u;
         }
         __syncwarp();
         tc_commit_elect(&sh.done);
