@@ -107,6 +107,13 @@ __device__ __forceinline__ void fma_two(uint64_t& sum, uint64_t s, uint32_t x, u
     asm("{\n\t.reg .b64 v;\n\tmov.b64 v, {%2, %3};\n\tfma.rn.f32x2 %0, %1, v, %0;\n\t}" : "+l"(sum) : "l"(s), "r"(x), "r"(y));
 }
 
+// mbar_poll that does not wait
+__device__ __forceinline__ uint32_t mbar_test(uint32_t bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok;
+}
 // (mbar_wait_warp with its slow part in line: a call would take the registers that the sums are in)
 __device__ __forceinline__ bool wait_bar_slow(uint32_t bar, uint32_t parity, PfWaits* waits)
 {
@@ -234,6 +241,7 @@ __global__ void __launch_bounds__((WgPlan<GROUPS, TOKENS>::kThreads), 1) w4_gemm
         const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + t0;
         uint64_t sum[kColumns / 2];                       // two tokens in each
         Ring<2> acc;
+        uint32_t ready = 0;                               // the accumulator was there when last looked at
         bool ok = true;
         for (int i = i0; i < i1 && ok; ++i, now.next(blocks, sh.first, a.E, passes))
         {
@@ -241,57 +249,61 @@ __global__ void __launch_bounds__((WgPlan<GROUPS, TOKENS>::kThreads), 1) w4_gemm
             const int rows = rows_of(now, base);
             const size_t unit = ((size_t)now.e * a.S + min(now.block * 8 + r / 16, a.S - 1)) * a.C;
             const uint16_t* sc = a.sc + (unit + c0) * 16 * GROUPS + (r & 7) * 2 * GROUPS + (r >> 3 & 1);
-            // scales two chunks ahead
-            uint16_t next[2][GROUPS];
+            // scales of the next chunks; a place is loaded again when its chunk is through (moved from place to place, a scale would be waited for by the move)
+            constexpr int kAhead = GROUPS == 4 ? 2 : 4;
+            uint16_t next[kAhead][GROUPS];
 #pragma unroll
-            for (int d = 0; d < 2; ++d)
+            for (int d = 0; d < kAhead; ++d)
 #pragma unroll
                 for (int j = 0; j < GROUPS; ++j) next[d][j] = c0 + d < c1 ? sc[d * 16 * GROUPS + 2 * j] : 0;
 #pragma unroll
             for (int j = 0; j < kColumns / 2; ++j) sum[j] = 0;
-            for (int c = c0; c < c1 && ok; ++c)
-            {
-                uint16_t scale[GROUPS];
-                sc += 16 * GROUPS;
+#pragma unroll 1
+            for (int c = c0; c < c1 && ok; c += kAhead)
 #pragma unroll
-                for (int j = 0; j < GROUPS; ++j)
+                for (int d = 0; d < kAhead; ++d)
                 {
-                    scale[j] = next[0][j];
-                    next[0][j] = next[1][j];
-                    next[1][j] = c + 2 < c1 ? sc[16 * GROUPS + 2 * j] : 0;
-                }
+                    if (c + d >= c1) break;
+                    sc += 16 * GROUPS;
+                    uint64_t scale[GROUPS];
 #pragma unroll
-                for (int j0 = 0; j0 < GROUPS; j0 += Plan::kSet)
-                {
-                    ok = ok && wait_bar(saddr(&sh.sum_full[acc.s]), acc.parity, &sh.waits);
-                    if (!ok) break;
-                    tc_fence_after();
-                    constexpr int kAtOnce = kColumns < 32 ? kColumns : 32;
-#pragma unroll
-                    for (int j = 0; j < Plan::kSet; ++j)
+                    for (int j = 0; j < GROUPS; ++j)
                     {
-                        const uint64_t s = two_floats(scales_of<SC>(scale[j0 + j]).x);
-#pragma unroll
-                        for (int k0 = 0; k0 < kColumns; k0 += kAtOnce)
-                        {
-                            uint32_t v[kAtOnce / 16][16];
-#pragma unroll
-                            for (int h = 0; h < kAtOnce / 16; ++h) tmem_ld16_async(from + acc.s * Plan::kSumColumns + j * TOKENS + k0 + 16 * h, v[h]);
-#pragma unroll
-                            for (int h = 0; h < kAtOnce / 16; ++h) tmem_wait_ld(v[h]);
-                            if (k0 + kAtOnce == kColumns && j == Plan::kSet - 1)
-                            {
-                                tc_fence_before();
-                                __syncwarp();
-                                if (lane == 0) mbar_arrive(&sh.sum_empty[acc.s]);
-                            }
-#pragma unroll
-                            for (int k = 0; k < kAtOnce / 2; ++k) fma_two(sum[k0 / 2 + k], s, v[k / 8][2 * k % 16], v[k / 8][2 * k % 16 + 1]);
-                        }
+                        scale[j] = two_floats(scales_of<SC>(next[d][j]).x);
+                        if (c + d + kAhead < c1) next[d][j] = sc[(kAhead - 1) * 16 * GROUPS + 2 * j];
                     }
-                    acc.next();
+#pragma unroll
+                    for (int j0 = 0; j0 < GROUPS; j0 += Plan::kSet)
+                    {
+                        if (__builtin_expect(!__all_sync(0xffffffffu, ready), 0)) ok = ok && wait_bar_slow(saddr(&sh.sum_full[acc.s]), acc.parity, &sh.waits);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t at = from + acc.s * Plan::kSumColumns, sum_empty = saddr(&sh.sum_empty[acc.s]);
+                        acc.next();
+                        constexpr int kAtOnce = kColumns < 32 ? kColumns : 32;
+#pragma unroll
+                        for (int j = 0; j < Plan::kSet; ++j)
+#pragma unroll
+                            for (int k0 = 0; k0 < kColumns; k0 += kAtOnce)
+                            {
+                                uint32_t v[kAtOnce / 16][16];
+#pragma unroll
+                                for (int h = 0; h < kAtOnce / 16; ++h) tmem_ld16_async(at + j * TOKENS + k0 + 16 * h, v[h]);
+#pragma unroll
+                                for (int h = 0; h < kAtOnce / 16; ++h) tmem_wait_ld(v[h]);
+                                if (k0 + kAtOnce == kColumns && j == Plan::kSet - 1)
+                                {
+                                    tc_fence_before();
+                                    __syncwarp();
+                                    if (lane == 0) mbar_arrive32(sum_empty);
+                                    ready = mbar_test(saddr(&sh.sum_full[acc.s]), acc.parity);      // of the next accumulator, behind the products
+                                }
+#pragma unroll
+                                for (int k = 0; k < kAtOnce / 2; ++k) fma_two(sum[k0 / 2 + k], scale[j0 + j], v[k / 8][2 * k % 16], v[k / 8][2 * k % 16 + 1]);
+                            }
+                    }
+                    if (!ok) break;
                 }
-            }
             if (ck == 1 && ok)
             {
                 const int n = now.block * 128 + r, there = n < a.N ? rows - t0 : 0;
