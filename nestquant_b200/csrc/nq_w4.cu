@@ -1,4 +1,6 @@
 // Products with 4-bit weights (nq_w4.cuh): the layout of the planes, and the kernel for calls of few rows.
+#include <limits.h>
+
 #include "nq_tc.cuh"
 #include "nq_w4.cuh"
 
@@ -166,6 +168,7 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) w4_kernel(W4 a)
     else
     {
         grid_dependency_wait();
+        if (w4_other_call(a)) return;
         passes = expert_passes<kRows>(a, s_row, s_first, s_warp);
         zero_rows_behind(a, s_row[a.E]);
     }
@@ -277,7 +280,7 @@ __global__ void __launch_bounds__(32 * kW4Warps, 1) w4_kernel(W4 a)
     add_up(s_part + ((i1 - 1) & 1) * Plan::kPart, old_block, old_base, old_rows);
 }
 
-int w4_gemm(const W4& a, int type, int sc_type, int group, int device, cudaStream_t st);       // nq_w4_gemm.cu
+int w4_gemm(const W4& a, int tokens, int type, int sc_type, int group, int device, cudaStream_t st);       // nq_w4_gemm.cu
 
 bool w4_shape(int E, int N, int K, int g)
 {
@@ -292,10 +295,6 @@ int w4_pitch(int C, int ck) { return ((C + ck - 1) / ck) * 256 + 64; }
 // How a matrix is cut: CTAs of a cluster and warps of a CTA that share a strip, both powers of two.  The device takes ceil(blocks / clusters) rounds; a round
 // costs a warp its units and what comes per item (sums and barriers: as much as a unit and a half, over a cluster three).  Rows of x weigh in so that 8 rows of
 // 6,144 columns, 98 KB for each CTA of its own, are shared by two CTAs: 7.6 us instead of 8.2.
-// Calls for the other kernel.  us, this kernel / that one, 4,096 x 6,144: 16 rows 9.5 / 11.3, 32 rows (four tiles here) 15.4 / 10.8; 6,144 x 2,048 in groups of 64:
-// 7.2 / 9.8, 11.4 / 9.8; 16,384 x 8,192, 16 rows: 27 / 37.
-bool w4_many_rows(int rows, int E, const int* start) { return (start ? rows / E : rows) > 16; }
-
 template <class X, class SC, int GROUPS, int TILES>
 bool w4_cut(W4& a, int rows, int device, cudaLaunchConfig_t& cfg, long long& clusters)
 {
@@ -343,7 +342,8 @@ int w4_launch(W4 a, int device, cudaStream_t st)
     cfg.blockDim = dim3(32 * kW4Warps); cfg.stream = st;
     long long clusters;
     if (!w4_cut<X, SC, GROUPS, TILES>(a, rows, device, cfg, clusters)) return fail(NQ_ERR_ARG, "nq_w4_matmul: no room for %d rows of %d columns", rows, a.K);
-    const long long most = (long long)a.blocks * (a.start ? a.rows / (8 * TILES) + (a.E < a.rows ? a.E : a.rows) : (a.rows - 1) / (8 * TILES) + 1);
+    const int of = a.rows < a.upto ? a.rows : a.upto;          // rows that experts may have here
+    const long long most = (long long)a.blocks * (a.start ? of / (8 * TILES) + (a.E < of ? a.E : of) : (a.rows - 1) / (8 * TILES) + 1);
     NQ_REQUIRE(most <= 0x7fffffff / a.C, "nq_w4_matmul: %d rows are too many", a.rows);       // (units are counted in 32 bits)
     if (most < clusters) clusters = most;
     attr[0].val.clusterDim.x = 1 << a.log_ck;
@@ -356,15 +356,19 @@ int w4_launch(W4 a, int device, cudaStream_t st)
 template <class X, class SC, int GROUPS>
 int w4_tiles(const W4& a, int device, cudaStream_t st)
 {
-    // one tile of eight rows where the call, or an expert on average, has no more, or shared memory does not hold sixteen; else two
-    const int rows = a.start ? a.rows / a.E : a.rows;
-    if (rows <= 8 || 16 * w4_pitch(a.C, a.C < 8 ? a.C : 8) > W4Plan<GROUPS, 2>::kRoom) return w4_launch<X, SC, GROUPS, 1>(a, device, st);
+    // one tile of eight rows where the call has no more, or an expert on average, or shared memory does not hold sixteen; else two
+    if (a.start || a.rows <= 8 || 16 * w4_pitch(a.C, a.C < 8 ? a.C : 8) > W4Plan<GROUPS, 2>::kRoom) return w4_launch<X, SC, GROUPS, 1>(a, device, st);
     return w4_launch<X, SC, GROUPS, 2>(a, device, st);
 }
 template <class X, class SC>
 int w4_groups(const W4& a, int g, int device, cudaStream_t st)
 {
     return g == 128 ? w4_tiles<X, SC, 1>(a, device, st) : g == 64 ? w4_tiles<X, SC, 2>(a, device, st) : w4_tiles<X, SC, 4>(a, device, st);
+}
+int w4_few(const W4& a, int type, int sc_type, int group, int device, cudaStream_t st)
+{
+    if (type == NQ_F16) return sc_type == NQ_F16 ? w4_groups<__half, __half>(a, group, device, st) : w4_groups<__half, __nv_bfloat16>(a, group, device, st);
+    return sc_type == NQ_F16 ? w4_groups<__nv_bfloat16, __half>(a, group, device, st) : w4_groups<__nv_bfloat16, __nv_bfloat16>(a, group, device, st);
 }
 
 }  // namespace nq
@@ -402,14 +406,30 @@ int nq_w4_matmul(const void* x, int type, long long x_stride, const void* qw, co
     NQ_REQUIRE(x && qw && sc && out && status, "nq_w4_matmul: null pointer");
     NQ_REQUIRE(nq::aligned16(x) && x_stride % 8 == 0 && nq::aligned16(qw) && nq::aligned16(sc), "nq_w4_matmul: rows of x and planes start on 16 bytes");
     nq::W4 a{(const uint4*)qw, (const uint16_t*)sc, (const uint8_t*)zp, x, start, out, status, x_stride, out_stride, rows, N, K, E, nq::w4_strips(N), nq::w4_chunks(K),
-             out_type, 0, 0, 0, 0, 0};
+             out_type, 0, 0, 0, 0, 0, INT_MIN, INT_MAX};
     int device;
     if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&a.sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
         return nq::fail(NQ_ERR_CUDA, "nq_w4_matmul: no device");
     cudaStream_t st = (cudaStream_t)stream;
-    if (nq::w4_many_rows(rows, E, start)) return nq::w4_gemm(a, type, sc_type, group, device, st);
-    if (type == NQ_F16) return sc_type == NQ_F16 ? nq::w4_groups<__half, __half>(a, group, device, st) : nq::w4_groups<__half, __nv_bfloat16>(a, group, device, st);
-    return sc_type == NQ_F16 ? nq::w4_groups<__nv_bfloat16, __half>(a, group, device, st) : nq::w4_groups<__nv_bfloat16, __nv_bfloat16>(a, group, device, st);
+    // This kernel or that of nq_w4_gemm.cu, us: 9.0 / 9.5 with 12 rows of 4,096 x 6,144, 9.4 / 9.5 with 16, 15.4 / 9.7 with 32 (four tiles here); of 6,144 x 2,048 in groups of
+    // 64, 7.5 / 7.2, 7.7 / 7.3, 11.4 / 7.4; of 16,384 x 8,192, 24.9 / 25.1, 26.7 / 25.1.
+    if (!start) return rows > 16 ? nq::w4_gemm(a, rows <= 32 ? 32 : rows <= 64 ? 64 : 128, type, sc_type, group, device, st) : nq::w4_few(a, type, sc_type, group, device, st);
+    // Experts' numbers of rows differ, and one of nine takes two passes here.  32 experts of 4,096 x 6,144 with 4, 8, 12 rows on average: 95 / 111, 136 / 132, 155 / 133;
+    // 128 of 2,048 x 2,048: 68 / 71, 101 / 81, 129 / 94; 64 of 2,048 x 4,096 in groups of 32: 75 / 92, 108 / 101, 117 / 107.  There, an expert of one and a half times the
+    // average should not take two passes, of 32, 64 or 128 rows.  A launch that ends at once costs 0.5 us here, 2.3 there: the one for items of 32 rows is made
+    // in the place of others for 64 MB of planes or more, which take 20 or longer (an eighth of 64 and 128 rows for each of the 32 experts: 170 -> 133, 200 -> 155).
+    const int few = 8 * E, some = 64 * E / 3, tokens = rows <= some ? 32 : rows <= 2 * some ? 64 : 128;
+    auto launch = [&](int form, int upto) {
+        a.upto = rows <= upto ? INT_MAX : upto;
+        const int e = form ? nq::w4_gemm(a, form, type, sc_type, group, device, st) : nq::w4_few(a, type, sc_type, group, device, st);
+        a.more = a.upto;
+        return e;
+    };
+    a.more = INT_MIN;
+    int e = launch(0, few);
+    if (!e && a.more != INT_MAX && tokens > 32 && (int64_t)E * a.S * a.C >= 65536) e = launch(32, some);
+    if (!e && a.more != INT_MAX) e = launch(tokens, INT_MAX);
+    return e;
 }
 
 }  // extern "C"

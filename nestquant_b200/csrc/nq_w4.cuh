@@ -32,6 +32,7 @@ struct W4 {
     long long x_stride, out_stride;
     int rows, N, K, E, S, C, out_type;
     int log_ck, log_wk, pitch, blocks, sms;         // see w4_kernel
+    int more, upto;                                 // see w4_other_call
 };
 
 // c = a b, or c += a b: a sum that starts does not need zeros in registers
@@ -233,6 +234,13 @@ __device__ __forceinline__ int expert_passes(const W4& a, int* row, int* first, 
     if (falls && blockIdx.x == 0 && threadIdx.x == 0) *a.status = 2;
     __syncthreads();
     return passes;
+}
+// How many rows the experts have stands in start[E], on the device: `rows` only bounds it, by eight times as much where other ranks have most picks.  Of the launches
+// of a call, one for each form that may be the best for it, the one with more < start[E] <= upto does the work; the others end at once.
+__device__ __forceinline__ bool w4_other_call(const W4& a)
+{
+    const int rows = a.start[a.E];
+    return rows <= a.more || rows > a.upto;
 }
 // zeros into the rows that no expert has
 __device__ __forceinline__ void zero_rows_behind(const W4& a, int behind)

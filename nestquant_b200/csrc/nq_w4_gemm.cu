@@ -7,11 +7,13 @@
 //   TMA        (one warp) the tokens' tiles [TOKENS x 64], two per chunk of 128 columns
 //   MMAs       (one warp) an elected lane issues tcgen05.mma, 128 x TOKENS x 16 a step, into one of two accumulators per group of columns: an accumulator
 //              holds one group's sum only, so that the scale is applied in 32 bits and nothing is rounded before the result
-// Bound by the tensor pipe by intent; in practice by the tokens' tiles from L2 (each CTA reads its own: 37 bytes per clock and SM at 512 rows) and by the issue slots that
-// weights and sums share with the MMAs.  us, rows of 4,096 x 6,144 in groups of 128 (tensor floor): 32 10.8, 64 12.2, 128 14.3 (3.9), 512 28.5 (15.7), 2,048 105
-// (62.8) = 0.98 PFLOP/s; in groups of 32, 512 rows, 65: four times the sums.  What made the difference at 512 rows: one row block of 32 per pass of the other kernel
-// 156; this kernel with eight warps of 128 tokens' sums and the MMAs one by one 35; registers by role and two sums an instruction 30.  Passes of up to 64 rows: an MMA of
-// 16 columns takes ~56 clocks however few tokens it has, and sixteen warps decode.
+// Bound by the tensor pipe by intent; in practice at 128 rows an item by the sums, which read 128 x 128 of tensor memory a chunk, and the MMAs, which wait for
+// them with two accumulators: a chunk takes 820 clocks, 512 of them MMAs; weights are three chunks ahead.  us, rows of 4,096 x 6,144 in groups of 128 (tensor floor):
+// 32 9.7, 64 10.9, 128 13.3 (3.9), 256 18.0 (7.8), 512 24.6 (15.7), 2,048 97 (62.8) = 1.06 PFLOP/s; 512 rows in groups of 64 33.5, of 32 55: two and four times the sums.
+// What made the difference at 512 rows: one row block of 32 per pass of the other kernel 156; this kernel with eight warps of 128 tokens' sums and the MMAs one by one
+// 35; registers by role and two sums an instruction 30; one vote for a chunk's three barriers 24.6.  In groups of 64: scales that stay where they were loaded and the
+// next barrier looked at behind the products 36.5 -> 33.5.  Passes of up to 64 rows: an MMA of 16 columns takes ~56 clocks however few tokens it has, and sixteen warps
+// decode.
 // Columns of an item may be split over a cluster; each CTA then adds up a share of the tokens, the others' sums come through distributed shared memory.
 // Every mbarrier wait is bounded (nq_tc.cuh): on time-out the CTA raises status[0], waits for its loads and MMAs in flight and ends.
 #include <stddef.h>
@@ -202,6 +204,11 @@ __global__ void __launch_bounds__((WgPlan<GROUPS, TOKENS>::kThreads), 1) w4_gemm
         sh.waits.aborted = 0; sh.waits.limit_ns = (unsigned long long)kPfWaitNs;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (a.start)
+    {
+        grid_dependency_wait();
+        if (w4_other_call(a)) return;
+    }
     if (warp == Plan::kMma)
     {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(&sh.tmem)), "r"(512) : "memory");
@@ -215,7 +222,6 @@ __global__ void __launch_bounds__((WgPlan<GROUPS, TOKENS>::kThreads), 1) w4_gemm
     }
     else
     {
-        grid_dependency_wait();
         passes = expert_passes<TOKENS>(a, sh.row, sh.first, sh.warp_sums);
         zero_rows_behind(a, sh.row[a.E]);
     }
@@ -547,7 +553,8 @@ int wg_launch(Wg g, int device, cudaStream_t st)
     auto* kernel = w4_gemm_kernel<X, SC, GROUPS, TOKENS>;
     if (!allow_shared<w4_gemm_kernel<X, SC, GROUPS, TOKENS>>(Plan::kSmem, device)) return fail(NQ_ERR_CUDA, "nq_w4_matmul: shared memory");
     a.blocks = (a.S - 1) / 8 + 1;
-    const long long most = (long long)a.blocks * (a.start ? a.rows / TOKENS + (a.E < a.rows ? a.E : a.rows) : (a.rows - 1) / TOKENS + 1);
+    const int of = a.rows < a.upto ? a.rows : a.upto;          // rows that experts may have here
+    const long long most = (long long)a.blocks * (a.start ? of / TOKENS + (a.E < of ? a.E : of) : (a.rows - 1) / TOKENS + 1);
     NQ_REQUIRE(most <= 0x7fffffff / a.C, "nq_w4_matmul: %d rows are too many", a.rows);
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
@@ -573,24 +580,22 @@ int wg_launch(Wg g, int device, cudaStream_t st)
     return check_launch("nq_w4_matmul");
 }
 template <class X, class SC, int GROUPS>
-int wg_tokens(const Wg& g, int device, cudaStream_t st)
+int wg_tokens(const Wg& g, int tokens, int device, cudaStream_t st)
 {
-    const int rows = g.w.start ? g.w.rows / g.w.E * 3 / 2 : g.w.rows;      // (an expert of one and a half times the average should not take two passes)
-    if (rows <= 32) return wg_launch<X, SC, GROUPS, 32>(g, device, st);
-    if (rows <= 64) return wg_launch<X, SC, GROUPS, 64>(g, device, st);
-    return wg_launch<X, SC, GROUPS, 128>(g, device, st);
+    return tokens == 32 ? wg_launch<X, SC, GROUPS, 32>(g, device, st) : tokens == 64 ? wg_launch<X, SC, GROUPS, 64>(g, device, st) : wg_launch<X, SC, GROUPS, 128>(g, device, st);
 }
 template <class X, class SC>
-int wg_groups(const Wg& g, int group, int device, cudaStream_t st)
+int wg_groups(const Wg& g, int tokens, int group, int device, cudaStream_t st)
 {
-    return group == 128 ? wg_tokens<X, SC, 1>(g, device, st) : group == 64 ? wg_tokens<X, SC, 2>(g, device, st) : wg_tokens<X, SC, 4>(g, device, st);
+    return group == 128 ? wg_tokens<X, SC, 1>(g, tokens, device, st) : group == 64 ? wg_tokens<X, SC, 2>(g, tokens, device, st) : wg_tokens<X, SC, 4>(g, tokens, device, st);
 }
 
-int w4_gemm(const W4& a, int type, int sc_type, int group, int device, cudaStream_t st)
+// with items of `tokens` rows of x: 32, 64 or 128
+int w4_gemm(const W4& a, int tokens, int type, int sc_type, int group, int device, cudaStream_t st)
 {
     const Wg g{a, 0};
-    if (type == NQ_F16) return sc_type == NQ_F16 ? wg_groups<__half, __half>(g, group, device, st) : wg_groups<__half, __nv_bfloat16>(g, group, device, st);
-    return sc_type == NQ_F16 ? wg_groups<__nv_bfloat16, __half>(g, group, device, st) : wg_groups<__nv_bfloat16, __nv_bfloat16>(g, group, device, st);
+    if (type == NQ_F16) return sc_type == NQ_F16 ? wg_groups<__half, __half>(g, tokens, group, device, st) : wg_groups<__half, __nv_bfloat16>(g, tokens, group, device, st);
+    return sc_type == NQ_F16 ? wg_groups<__nv_bfloat16, __half>(g, tokens, group, device, st) : wg_groups<__nv_bfloat16, __nv_bfloat16>(g, tokens, group, device, st);
 }
 
 }  // namespace nq

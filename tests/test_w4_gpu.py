@@ -91,6 +91,62 @@ def test_a_matrix_per_expert(sizes, extra, N, K, g, dtype, out, zeros):
     assert (y[int(start[-1]):] == 0).all()
 
 
+@pytest.mark.parametrize("dtype,g", [(F16, 128), (BF16, 32)])
+def test_the_number_of_rows_is_the_devices(dtype, g):
+    """a captured call whose start array has few rows, then many, then none, then one that falls: whichever form of the product takes it, rows behind are zero"""
+    from nestquant_b200 import w4
+    E, N, K, P = 5, 100, 384, 90
+    q, s, z = make(N, K, g, dtype, True, E=E, seed=3)
+    w = w4.W4(q, s, z)
+    x = torch.randn(P, K, generator=torch.Generator("cuda").manual_seed(8), device="cuda").to(dtype)
+    start = rows_of([1, 2, 3, 0, 1], E)[0]
+    w(x, start=start)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = w(x, start=start, dtype=F32)
+    for sizes in ([1, 2, 3, 0, 1], [10, 8, 0, 13, 9], [9, 0, 31, 0, 1], [18, 18, 18, 18, 18], [0, 0, 0, 0, 0], [0, 0, 39, 1, 0], [90, 0, 0, 0, 0], [0, 0, 0, 0, 7]):
+        start.copy_(rows_of(sizes, E)[0])
+        y.fill_(float("nan"))
+        graph.replay()
+        for e in range(E):
+            a, b = int(start[e]), int(start[e + 1])
+            if a < b:
+                check(y[a:b], x[a:b], dense(q[e], s[e], z[e], g), K)
+        assert (y[int(start[-1]):] == 0).all(), sizes
+    for last in (30, 60):
+        start.copy_(torch.tensor([0, 9, 8, 12, 20, last], dtype=torch.int32))
+        y.fill_(float("nan"))
+        graph.replay()
+        assert (y == 0).all()
+
+
+def test_the_number_of_rows_is_the_devices_with_64_mb_of_planes():
+    """likewise, where calls of few rows an expert have a form of their own between the smallest and the call's bound"""
+    from nestquant_b200 import w4
+    E, N, K, g, P = 64, 1024, 2048, 64, 64 * 45
+    q, s, z = make(N, K, g, F16, False, E=E, seed=3)
+    w = w4.W4(q, s)
+    x = torch.randn(P, K, generator=torch.Generator("cuda").manual_seed(8), device="cuda").half()
+    start = torch.zeros(E + 1, dtype=torch.int32, device="cuda")
+    w(x, start=start)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = w(x, start=start, dtype=F32)
+    gen = torch.Generator().manual_seed(1)
+    for total in (0, 1, 512, 513, 1365, 1366, P - 1, P):        # 8 and 64 / 3 rows an expert, and one more
+        cuts = torch.cat([torch.zeros(1), torch.randint(0, total + 1, (E - 1,), generator=gen).sort()[0], torch.full((1,), total)]).int()
+        start.copy_(cuts)
+        y.fill_(float("nan"))
+        graph.replay()
+        for e in range(E):
+            a, b = int(cuts[e]), int(cuts[e + 1])
+            if a < b:
+                check(y[a:b], x[a:b], dense(q[e], s[e], None, g), K)
+        assert (y[total:] == 0).all(), total
+
+
 def test_a_rows_bits_do_not_depend_on_the_others_in_its_call():
     """at the sizes of a decode call: the order of a row's sums goes by the matrix alone"""
     from nestquant_b200 import w4
