@@ -55,6 +55,10 @@ __global__ void __launch_bounds__(256) w4_layout_kernel(W4Layout a, unsigned uni
     }
 }
 
+// Products of a single matrix ask for planes before their predecessor's end has been waited for, when its writes need not be there.  Nothing starts this kernel early,
+// so that the layout's are when it runs.
+__global__ void w4_settled_kernel() {}
+
 // ---- product ------------------------------------------------------------------------------------------------------------------
 
 // acc += the unit's 16 x 128 weights times rows of x: xs[n] = shared address of the lane's row of tile n, its pieces of the unit's columns
@@ -391,6 +395,7 @@ int nq_w4_layout(const void* q, const void* scales, const void* zeros, int E, in
     NQ_REQUIRE((int64_t)E * S * C <= 0x7fffffff, "nq_w4_layout: too many units");
     const unsigned units = (unsigned)((int64_t)E * S * C);
     nq::w4_layout_kernel<<<(units - 1) / nq::kLayoutUnits + 1, 256, 0, (cudaStream_t)stream>>>(nq::W4Layout{(const uint8_t*)q, (const uint16_t*)scales, (const uint8_t*)zeros, (uint32_t*)qw, (uint16_t*)sc, (uint8_t*)zp, E, N, K, group, S, C}, units);
+    nq::w4_settled_kernel<<<1, 1, 0, (cudaStream_t)stream>>>();
     return nq::check_launch("nq_w4_layout");
 }
 
