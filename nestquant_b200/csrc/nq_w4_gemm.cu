@@ -286,27 +286,24 @@ __global__ void __launch_bounds__((WgPlan<GROUPS, TOKENS>::kThreads), 1) w4_gemm
                         tc_fence_after();
                         const uint32_t at = from + acc.s * Plan::kSumColumns, sum_empty = saddr(&sh.sum_empty[acc.s]);
                         acc.next();
-                        constexpr int kAtOnce = kColumns < 32 ? kColumns : 32;
 #pragma unroll
                         for (int j = 0; j < Plan::kSet; ++j)
+                        {
+                            uint32_t v[kColumns / 16][16];
 #pragma unroll
-                            for (int k0 = 0; k0 < kColumns; k0 += kAtOnce)
+                            for (int h = 0; h < kColumns / 16; ++h) tmem_ld16_async(at + j * TOKENS + 16 * h, v[h]);
+#pragma unroll
+                            for (int h = 0; h < kColumns / 16; ++h) tmem_wait_ld(v[h]);
+                            if (j == Plan::kSet - 1)
                             {
-                                uint32_t v[kAtOnce / 16][16];
-#pragma unroll
-                                for (int h = 0; h < kAtOnce / 16; ++h) tmem_ld16_async(at + j * TOKENS + k0 + 16 * h, v[h]);
-#pragma unroll
-                                for (int h = 0; h < kAtOnce / 16; ++h) tmem_wait_ld(v[h]);
-                                if (k0 + kAtOnce == kColumns && j == Plan::kSet - 1)
-                                {
-                                    tc_fence_before();
-                                    __syncwarp();
-                                    if (lane == 0) mbar_arrive32(sum_empty);
-                                    ready = mbar_test(saddr(&sh.sum_full[acc.s]), acc.parity);      // of the next accumulator, behind the products
-                                }
-#pragma unroll
-                                for (int k = 0; k < kAtOnce / 2; ++k) fma_two(sum[k0 / 2 + k], scale[j0 + j], v[k / 8][2 * k % 16], v[k / 8][2 * k % 16 + 1]);
+                                tc_fence_before();
+                                __syncwarp();
+                                if (lane == 0) mbar_arrive32(sum_empty);
+                                ready = mbar_test(saddr(&sh.sum_full[acc.s]), acc.parity);      // of the next accumulator, behind the products
                             }
+#pragma unroll
+                            for (int k = 0; k < kColumns / 2; ++k) fma_two(sum[k], scale[j0 + j], v[k / 8][2 * k % 16], v[k / 8][2 * k % 16 + 1]);
+                        }
                     }
                     if (!ok) break;
                 }
