@@ -8,12 +8,12 @@
 //   MMAs       (one warp) an elected lane issues tcgen05.mma, 128 x TOKENS x 16 a step, into one of two accumulators per group of columns: an accumulator
 //              holds one group's sum only, so that the scale is applied in 32 bits and nothing is rounded before the result
 // Bound by the tensor pipe by intent; in practice at 128 rows an item by the sums, which read 128 x 128 of tensor memory a chunk, and the MMAs, which wait for
-// them with two accumulators: a chunk takes 820 clocks, 512 of them MMAs; weights are three chunks ahead.  us, rows of 4,096 x 6,144 in groups of 128 (tensor floor):
-// 32 9.7, 64 10.9, 128 13.3 (3.9), 256 18.0 (7.8), 512 24.6 (15.7), 2,048 97 (62.8) = 1.06 PFLOP/s; 512 rows in groups of 64 33.5, of 32 55: two and four times the sums.
-// What made the difference at 512 rows: one row block of 32 per pass of the other kernel 156; this kernel with eight warps of 128 tokens' sums and the MMAs one by one
-// 35; registers by role and two sums an instruction 30; one vote for a chunk's three barriers 24.6.  In groups of 64: scales that stay where they were loaded and the
-// next barrier looked at behind the products 36.5 -> 33.5.  Passes of up to 64 rows: an MMA of 16 columns takes ~56 clocks however few tokens it has, and sixteen warps
-// decode.
+// one another over two accumulators: a chunk takes 820 clocks, 512 of them MMAs; weights are three chunks ahead.  us, rows of 4,096 x 6,144 in groups of 128 (tensor
+// floor): 32 9.4, 64 11.0, 128 13.4 (3.9), 256 18.0 (7.8), 512 24.3 (15.7), 2,048 95 (62.8) = 1.08 PFLOP/s; 512 rows in groups of 64 35, of 32 55: two and four times the
+// sums.  What made the difference at 512 rows: one row block of 32 per pass of the other kernel 156; this kernel with eight warps of 128 tokens' sums and the MMAs one by
+// one 35; registers by role and two sums an instruction 30; one vote for a chunk's three barriers 24.6.  In groups of 64: scales that stay where they were loaded and
+// the next barrier looked at behind the products 36.5 -> 33.5; in groups of 32: an accumulator read at once 58 -> 55.  Passes of up to 64 rows: an MMA of 16 columns takes
+// ~56 clocks however few tokens it has, and sixteen warps decode.
 // Columns of an item may be split over a cluster; each CTA then adds up a share of the tokens, the others' sums come through distributed shared memory.
 // Every mbarrier wait is bounded (nq_tc.cuh): on time-out the CTA raises status[0], waits for its loads and MMAs in flight and ends.
 #include <stddef.h>
