@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(kRowsThreads) combine_bwd_kernel(CombineBwd a)
             w[k] = k < n && p[k] < live ? load_as(a.rw, a.rw_type, pick + k) : 0.f;
         }
         if (there)
-            for (int v = r; v < a.pieces; v += per)
+            for (unsigned v = r; v < (unsigned)a.pieces; v += per)      // (a row may have 2^31 - 1)
             {
                 float d[N];
                 Piece<Y, N> y[kPicks];

@@ -411,7 +411,7 @@ int nq_w4_matmul(const void* x, int type, long long x_stride, const void* qw, co
     NQ_REQUIRE(x && qw && sc && out && status, "nq_w4_matmul: null pointer");
     NQ_REQUIRE(nq::aligned16(x) && x_stride % 8 == 0 && nq::aligned16(qw) && nq::aligned16(sc), "nq_w4_matmul: rows of x and planes start on 16 bytes");
     nq::W4 a{(const uint4*)qw, (const uint16_t*)sc, (const uint8_t*)zp, x, start, out, status, x_stride, out_stride, rows, N, K, E, nq::w4_strips(N), nq::w4_chunks(K),
-             out_type, 0, 0, 0, 0, 0, INT_MIN, INT_MAX};
+             out_type, 0, 0, 0, 0, 0, -1, INT_MAX};
     int device;
     if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&a.sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess)
         return nq::fail(NQ_ERR_CUDA, "nq_w4_matmul: no device");
@@ -430,7 +430,6 @@ int nq_w4_matmul(const void* x, int type, long long x_stride, const void* qw, co
         a.more = a.upto;
         return e;
     };
-    a.more = INT_MIN;
     int e = launch(0, few);
     if (!e && a.more != INT_MAX && tokens > 32 && (int64_t)E * a.S * a.C >= 65536) e = launch(32, some);
     if (!e && a.more != INT_MAX) e = launch(tokens, INT_MAX);

@@ -239,14 +239,15 @@ __device__ __forceinline__ int expert_passes(const W4& a, int* row, int* first, 
 // of a call, one for each form that may be the best for it, the one with more < start[E] <= upto does the work; the others end at once.
 __device__ __forceinline__ bool w4_other_call(const W4& a)
 {
-    const int rows = a.start[a.E];
+    const int rows = max(a.start[a.E], 0);
     return rows <= a.more || rows > a.upto;
 }
 // zeros into the rows that no expert has
 __device__ __forceinline__ void zero_rows_behind(const W4& a, int behind)
 {
-    for (int r = behind + (int)blockIdx.x; r < a.rows; r += gridDim.x)
-        for (int n = threadIdx.x; n < a.N; n += blockDim.x) store_as(a.out, a.out_type, (size_t)r * a.out_stride + n, 0.f);
+    // (in 32 unsigned bits: a step behind 2^31 - 1 is no negative number)
+    for (unsigned r = behind + blockIdx.x; r < (unsigned)a.rows; r += gridDim.x)
+        for (unsigned n = threadIdx.x; n < (unsigned)a.N; n += blockDim.x) store_as(a.out, a.out_type, (size_t)r * a.out_stride + n, 0.f);
 }
 
 }  // namespace nq

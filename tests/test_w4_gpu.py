@@ -114,7 +114,7 @@ def test_the_number_of_rows_is_the_devices(dtype, g):
             if a < b:
                 check(y[a:b], x[a:b], dense(q[e], s[e], z[e], g), K)
         assert (y[int(start[-1]):] == 0).all(), sizes
-    for last in (30, 60):
+    for last in (30, 60, -2 ** 31):
         start.copy_(torch.tensor([0, 9, 8, 12, 20, last], dtype=torch.int32))
         y.fill_(float("nan"))
         graph.replay()
