@@ -8,8 +8,9 @@
 // All of it is bound by HBM: (1 + topk) rows a token in each direction, read or written once.  Every row is touched in the widest pieces, 16 bytes at most, that
 // pointers and strides allow.  In copy and sum a thread has one piece of a token's row and the topk pieces that belong to it, so that
 // topk independent loads or stores are in flight per thread (predicated loads: behind branches they went one by one, 80 us instead of 67); the gradient of combine
-// has warps per token for the dot products, eight picks at a time.  4,096 tokens x 8 picks x 6,144 bf16, us (floor at the copy's 6.54 TB/s): copy 72 (69), sums
-// 67 (69: part of the rows is still in L2), combine's gradient 140 (131); 5,001 x 4 x 1,000: 7.8, 11, 22 (7.7, 7.7, 13.8).
+// has warps per token for the dot products, two, four or eight picks at a time (with places for eight 5,001 x 4 x 1,000 took 11 and 22 us: the registers, and loads
+// under predicates that do not hold).  4,096 tokens x 8 picks x 6,144 bf16, us (floor at the copy's 6.54 TB/s): copy 72 (69), sums 66 (69: part of the rows is
+// still in L2), combine's gradient 140 (131); 5,001 x 4 x 1,000: 7.5, 8.8, 16.9 (7.7, 7.7, 13.8).
 #include <initializer_list>
 #include <type_traits>
 
@@ -18,7 +19,7 @@
 
 namespace nq {
 
-constexpr int kRowsThreads = 256, kPicks = 8;       // picks of a token at a time
+constexpr int kRowsThreads = 256;
 
 struct Rows {
     const void* src; void* dst;
@@ -117,7 +118,7 @@ struct Piece {
 };
 
 // dst[t] = sum over the token's picks of src[pos] (times rw): dx of dispatch, out of combine
-template <class S, class D, int N, bool WEIGHTED>
+template <class S, class D, int N, int PICKS, bool WEIGHTED>
 __global__ void __launch_bounds__(kRowsThreads) sum_kernel(Rows a)
 {
     early_signal();
@@ -131,16 +132,16 @@ __global__ void __launch_bounds__(kRowsThreads) sum_kernel(Rows a)
     const size_t pick = t * a.topk;
     const S* src = (const S*)a.src + (size_t)v * N;
     float sum[N] = {};
-    for (int k0 = 0; k0 < a.topk; k0 += kPicks)
+    for (int k0 = 0; k0 < a.topk; k0 += PICKS)
     {
-        int p[kPicks];
-        Piece<S, N> x[kPicks];
+        int p[PICKS];
+        Piece<S, N> x[PICKS];
 #pragma unroll
-        for (int k = 0; k < kPicks; ++k) p[k] = k0 + k < a.topk ? a.pos[pick + k0 + k] : 0x7fffffff;
+        for (int k = 0; k < PICKS; ++k) p[k] = k0 + k < a.topk ? a.pos[pick + k0 + k] : 0x7fffffff;
 #pragma unroll
-        for (int k = 0; k < kPicks; ++k) x[k].load(src + (size_t)p[k] * a.H, p[k] < live);
+        for (int k = 0; k < PICKS; ++k) x[k].load(src + (size_t)p[k] * a.H, p[k] < live);
 #pragma unroll
-        for (int k = 0; k < kPicks; ++k)
+        for (int k = 0; k < PICKS; ++k)
         {
             if (p[k] >= live) continue;
             const float w = WEIGHTED ? load_as(a.rw, a.rw_type, pick + k0 + k) : 1.f;
@@ -158,25 +159,25 @@ struct CombineBwd {
     int warps;                                      // per token: 1, 2, 4 or 8
 };
 
-// dy and drw.  Y: type of y and dy, O: of dout, N elements at a time
-template <class Y, class O, int N>
+// dy and drw.  Y: type of y and dy, O: of dout, N elements and PICKS picks at a time
+template <class Y, class O, int N, int PICKS>
 __global__ void __launch_bounds__(kRowsThreads) combine_bwd_kernel(CombineBwd a)
 {
     early_signal();
     grid_dependency_wait();
-    __shared__ float s_dot[kRowsThreads / 32][kPicks];
+    __shared__ float s_dot[kRowsThreads / 32][PICKS];
     const int per = 32 * a.warps, slot = threadIdx.x / per, r = threadIdx.x % per, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const size_t t = (size_t)blockIdx.x * (kRowsThreads / per) + slot;
     const bool there = t < (size_t)a.T;             // every thread passes the barriers
     const int live = *a.live;
-    for (int k0 = 0; k0 < a.topk; k0 += kPicks)
+    for (int k0 = 0; k0 < a.topk; k0 += PICKS)
     {
-        int p[kPicks];
-        float w[kPicks], dot[kPicks] = {};
+        int p[PICKS];
+        float w[PICKS], dot[PICKS] = {};
         const size_t pick = t * a.topk + k0;
-        const int n = there ? min(kPicks, a.topk - k0) : 0;
+        const int n = there ? min(PICKS, a.topk - k0) : 0;
 #pragma unroll
-        for (int k = 0; k < kPicks; ++k)
+        for (int k = 0; k < PICKS; ++k)
         {
             p[k] = k < n ? a.pos[pick + k] : 0;
             w[k] = k < n && p[k] < live ? load_as(a.rw, a.rw_type, pick + k) : 0.f;
@@ -185,14 +186,14 @@ __global__ void __launch_bounds__(kRowsThreads) combine_bwd_kernel(CombineBwd a)
             for (unsigned v = r; v < (unsigned)a.pieces; v += per)      // (a row may have 2^31 - 1)
             {
                 float d[N];
-                Piece<Y, N> y[kPicks];
+                Piece<Y, N> y[PICKS];
                 if (a.drw)
 #pragma unroll
-                    for (int k = 0; k < kPicks; ++k) y[k].load((const Y*)a.y + (size_t)p[k] * a.H + (size_t)v * N, k < n && p[k] < live);
+                    for (int k = 0; k < PICKS; ++k) y[k].load((const Y*)a.y + (size_t)p[k] * a.H + (size_t)v * N, k < n && p[k] < live);
                 load_piece<O, N>((const O*)a.dout + t * a.H + (size_t)v * N, d);
                 if (a.dy)
 #pragma unroll
-                    for (int k = 0; k < kPicks; ++k)
+                    for (int k = 0; k < PICKS; ++k)
                     {
                         if (k >= n) continue;
                         float g[N];
@@ -202,14 +203,14 @@ __global__ void __launch_bounds__(kRowsThreads) combine_bwd_kernel(CombineBwd a)
                     }
                 if (a.drw)
 #pragma unroll
-                    for (int k = 0; k < kPicks; ++k)
+                    for (int k = 0; k < PICKS; ++k)
                         if (k < n && p[k] < live)
 #pragma unroll
                             for (int j = 0; j < N; ++j) dot[k] += y[k].at(j) * d[j];
             }
         if (!a.drw) continue;
 #pragma unroll
-        for (int k = 0; k < kPicks; ++k)
+        for (int k = 0; k < PICKS; ++k)
         {
             float s = dot[k];
 #pragma unroll
@@ -251,6 +252,15 @@ int row_grid(int T, int pieces, unsigned* grid, const char* what)
     return NQ_OK;
 }
 
+// picks of a token at a time: a few that a token does not have cost as much as those that it has
+template <class F>
+void by_picks(int topk, F&& launch)
+{
+    if (topk <= 2) launch(std::integral_constant<int, 2>());
+    else if (topk <= 4) launch(std::integral_constant<int, 4>());
+    else launch(std::integral_constant<int, 8>());
+}
+
 template <class S, class D, bool WEIGHTED>
 int sum_rows(Rows a, cudaStream_t st, const char* what)
 {
@@ -258,10 +268,13 @@ int sum_rows(Rows a, cudaStream_t st, const char* what)
     a.pieces = a.H / n;
     unsigned grid;
     if (int e = row_grid(a.T, a.pieces, &grid, what)) return e;
-    if (n == 8) { if constexpr (sizeof(S) == 2) launch_dependent(sum_kernel<S, D, 8, WEIGHTED>, dim3(grid), dim3(kRowsThreads), 0, st, a); }
-    else if (n == 4) launch_dependent(sum_kernel<S, D, 4, WEIGHTED>, dim3(grid), dim3(kRowsThreads), 0, st, a);
-    else if (n == 2) launch_dependent(sum_kernel<S, D, 2, WEIGHTED>, dim3(grid), dim3(kRowsThreads), 0, st, a);
-    else launch_dependent(sum_kernel<S, D, 1, WEIGHTED>, dim3(grid), dim3(kRowsThreads), 0, st, a);
+    by_picks(a.topk, [&](auto picks) {
+        constexpr int kP = decltype(picks)::value;
+        if (n == 8) { if constexpr (sizeof(S) == 2) launch_dependent(sum_kernel<S, D, 8, kP, WEIGHTED>, dim3(grid), dim3(kRowsThreads), 0, st, a); }
+        else if (n == 4) launch_dependent(sum_kernel<S, D, 4, kP, WEIGHTED>, dim3(grid), dim3(kRowsThreads), 0, st, a);
+        else if (n == 2) launch_dependent(sum_kernel<S, D, 2, kP, WEIGHTED>, dim3(grid), dim3(kRowsThreads), 0, st, a);
+        else launch_dependent(sum_kernel<S, D, 1, kP, WEIGHTED>, dim3(grid), dim3(kRowsThreads), 0, st, a);
+    });
     return check_launch(what);
 }
 
@@ -270,15 +283,18 @@ int combine_bwd(CombineBwd a, cudaStream_t st)
 {
     const int n = row_step<Y>(a.H, (int)(sizeof(O) > sizeof(Y) ? sizeof(O) : sizeof(Y)), {a.dout, a.y, a.dy});
     a.pieces = a.H / n;
-    // a warp per token if that makes 64 for each SM; more where there are few tokens and rows are long (3,000 x 6 x 4,096: 61 us, with 16 for each SM 70; eight
-    // always: 5,001 x 4 x 1,000 26 us instead of 22)
+    // a warp per token if that makes 64 for each SM; more where there are few tokens and rows are long (3,000 x 6 x 4,096: 67 us, with 16 for each SM 77, eight
+    // always 70; 5,001 x 4 x 1,000: 16.9, 17.3, 19.8)
     a.warps = 1;
     while (a.warps < 8 && 32 * a.warps < a.pieces && (long long)a.T * a.warps < 9472) a.warps *= 2;
     const int tokens = kRowsThreads / (32 * a.warps), grid = (a.T - 1) / tokens + 1;
-    if (n == 8) { if constexpr (sizeof(Y) == 2) launch_dependent(combine_bwd_kernel<Y, O, 8>, dim3(grid), dim3(kRowsThreads), 0, st, a); }
-    else if (n == 4) launch_dependent(combine_bwd_kernel<Y, O, 4>, dim3(grid), dim3(kRowsThreads), 0, st, a);
-    else if (n == 2) launch_dependent(combine_bwd_kernel<Y, O, 2>, dim3(grid), dim3(kRowsThreads), 0, st, a);
-    else launch_dependent(combine_bwd_kernel<Y, O, 1>, dim3(grid), dim3(kRowsThreads), 0, st, a);
+    by_picks(a.topk, [&](auto picks) {
+        constexpr int kP = decltype(picks)::value;
+        if (n == 8) { if constexpr (sizeof(Y) == 2) launch_dependent(combine_bwd_kernel<Y, O, 8, kP>, dim3(grid), dim3(kRowsThreads), 0, st, a); }
+        else if (n == 4) launch_dependent(combine_bwd_kernel<Y, O, 4, kP>, dim3(grid), dim3(kRowsThreads), 0, st, a);
+        else if (n == 2) launch_dependent(combine_bwd_kernel<Y, O, 2, kP>, dim3(grid), dim3(kRowsThreads), 0, st, a);
+        else launch_dependent(combine_bwd_kernel<Y, O, 1, kP>, dim3(grid), dim3(kRowsThreads), 0, st, a);
+    });
     return check_launch("nq_combine_bwd");
 }
 
