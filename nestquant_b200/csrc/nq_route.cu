@@ -380,7 +380,7 @@ struct RouteLaunch {
     {
         a.vec = run_aligned<L, PER>(a.logits, a.row_stride);
         a.vec_bias = run_aligned<float, PER>(a.bias, PER);
-        launch_dependent(route_kernel<L, PER>, dim3((a.T + kRouteWarps - 1) / kRouteWarps), dim3(32 * kRouteWarps), 0, st, a);
+        launch_dependent(route_kernel<L, PER>, dim3((a.T - 1) / kRouteWarps + 1), dim3(32 * kRouteWarps), 0, st, a);
     }
 };
 template <class L, int PER>
@@ -388,7 +388,7 @@ struct RouteBwdLaunch {
     static void go(RouteBwd a, cudaStream_t st)
     {
         a.vec = run_aligned<L, PER>(a.logits, a.row_stride) && run_aligned<L, PER>(a.dlogits, a.E);
-        launch_dependent(route_bwd_kernel<L, PER>, dim3((a.T + kRouteWarps - 1) / kRouteWarps), dim3(32 * kRouteWarps), 0, st, a);
+        launch_dependent(route_bwd_kernel<L, PER>, dim3((a.T - 1) / kRouteWarps + 1), dim3(32 * kRouteWarps), 0, st, a);
     }
 };
 
