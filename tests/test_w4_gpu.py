@@ -74,7 +74,7 @@ def rows_of(sizes, E, extra=0):
     return start, int(start[-1]) + extra
 
 
-@pytest.mark.parametrize("sizes,extra", [([0, 0, 0, 0, 0], 0), ([0, 0, 0, 0, 0], 3), ([1, 0, 2, 0, 1], 0), ([5, 8, 9, 0, 33], 7), ([0, 0, 0, 70, 0], 1), ([16, 17, 1, 3, 32], 40), ([30, 40, 20, 31, 29], 2), ([200, 1, 130, 0, 64], 0)])
+@pytest.mark.parametrize("sizes,extra", [([0, 0, 0, 0, 0], 0), ([0, 0, 0, 0, 0], 3), ([1, 0, 2, 0, 1], 0), ([5, 8, 9, 0, 33], 7), ([0, 0, 0, 70, 0], 1), ([16, 17, 1, 3, 32], 40), ([30, 40, 20, 31, 29], 2), ([200, 1, 130, 0, 64], 0), ([30], 5), ([3], 40), ([500], 0)])
 @pytest.mark.parametrize("N,K,g,dtype,out,zeros", [(48, 256, 128, F16, F16, False), (100, 352, 32, BF16, F32, True), (257, 1024, 64, BF16, BF16, True)])
 def test_a_matrix_per_expert(sizes, extra, N, K, g, dtype, out, zeros):
     from nestquant_b200 import w4
