@@ -86,7 +86,8 @@ int nq_promote(void* slot, const void* host_record, size_t record_bytes, int64_t
  *   pe [P] expert (or E) and pt [P] token of sorted pair p;  pos [P]: sorted index of pick t * topk + k;
  *   start [E + 2]: first pair of each bin (start[E] = number of live pairs, start[E + 1] = P);
  *   hit_counts [E] or NULL: += picks with a valid id and a non-zero weight, whatever the level (caller zeroes it; feed it to
- *   nq_pf_hits);  scratch: int32 [nq_pf_sort_scratch_ints(P, E)].
+ *   nq_pf_hits);  scratch: int32 [nq_pf_sort_scratch_ints(P, E)]: (E + 1) counts for every 256 pairs; 0 where that is more than
+ *   2^31 - 1, and the sort refuses such a call.
  * Replaces the host side of the reference's prefill (sm120/moe.py:293-298: argsort, scatter_add, .cpu() of the counts). */
 int nq_pf_sort_scratch_ints(int pairs, int E);
 int nq_pf_sort(const int64_t* sel, const void* rw, const int64_t* table, int T, int topk, int E, int32_t* pe, int32_t* pt,

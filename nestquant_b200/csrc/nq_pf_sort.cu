@@ -301,13 +301,15 @@ int sort_pairs(const int64_t* sel, const void* rw, const int64_t* table, int T, 
                int32_t* hits, int32_t* scratch, int scratch_ints, int32_t* plan, int plan_ints, void* stream)
 {
     NQ_REQUIRE(T >= 0 && topk >= 1 && E >= 1 && E + 1 <= kSortMaxBins, "nq_pf_sort: T = %d, topk = %d, E = %d", T, topk, E);
-    NQ_REQUIRE((long long)T * topk <= 0x7fffffffLL, "nq_pf_sort: too many pairs");
+    NQ_REQUIRE((long long)T * topk <= 0x7fffffffLL + 1 - kSortSlice, "nq_pf_sort: too many pairs");      // (a slice ends within 31 bits)
     const int P = T * topk;
     NQ_REQUIRE(start, "nq_pf_sort: null start array");
     cudaStream_t st = (cudaStream_t)stream;
     if (P == 0) return cudaMemsetAsync(start, 0, sizeof(int32_t) * (E + 2), st) == cudaSuccess ? NQ_OK : fail(NQ_ERR_CUDA, "nq_pf_sort: memset failed");
     NQ_REQUIRE(sel && !rw == !table && !pe == !pt && (pe || !table) && pos && scratch, "nq_pf_sort: null pointer");
-    NQ_REQUIRE(scratch_ints >= nq_pf_sort_scratch_ints(P, E), "nq_pf_sort: scratch needs %d ints", nq_pf_sort_scratch_ints(P, E));
+    const int ints = nq_pf_sort_scratch_ints(P, E);
+    NQ_REQUIRE(ints > 0, "nq_pf_sort: counts of %d x %d pairs and %d experts are more than an array can hold", T, topk, E);
+    NQ_REQUIRE(scratch_ints >= ints, "nq_pf_sort: scratch needs %d ints", ints);
     if (!table && P <= kSortIdsPicks) return sort_ids(sel, P, topk, E, pe, pt, pos, start, st);
     const size_t small = sizeof(int) * (33 * (size_t)(E + 1) + 1);
     if (P <= kSortSmallPicks && small <= kSortSmallShared)

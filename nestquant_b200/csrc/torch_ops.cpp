@@ -151,9 +151,10 @@ OrderPtr sort_picks(const Tensor& sel_, int64_t E)
     NQ_CHECK(sel_.scalar_type() == at::kLong, "sort_picks: sel, expected int64");
     const int64_t T = sel_.size(0), topk = sel_.size(1);
     NQ_CHECK(E >= 1 && E <= 1024 && topk >= 1 && 2 * T * topk + E + 2 <= 0x7fffffff, "sort_picks: ", T, " x ", topk, " picks of ", E, " experts (to 1024)");
+    const int ints = nq_pf_sort_scratch_ints((int)(T * topk), (int)E);
+    NQ_CHECK(ints > 0 || T == 0, "sort_picks: counts of ", T, " x ", topk, " picks and ", E, " experts are more than an array can hold");
     const c10::cuda::CUDAGuard guard(sel_.device());
     const Tensor sel = sel_.contiguous();
-    const int ints = nq_pf_sort_scratch_ints((int)(T * topk), (int)E);
     auto o = c10::make_intrusive<Order>();
     o->T = T; o->topk = topk; o->E = E;
     o->buf = at::empty({E + 2 + T * topk + std::max(ints, 1)}, sel.options().dtype(at::kInt));

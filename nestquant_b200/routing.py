@@ -32,7 +32,8 @@ def route(logits, topk, score="sigmoid", bias=None, renorm=True, scale=1.0, dtyp
 
 
 def sort_picks(sel, E):
-    """Expert ids int64 [T,topk] -> their Order: a stable sort by expert, picks whose id is outside [0, E) behind all others.  E <= 1024."""
+    """Expert ids int64 [T,topk] -> their Order: a stable sort by expert, picks whose id is outside [0, E) behind all others.  E <= 1024; somewhat
+    fewer than 2^30 picks, with 1,024 experts half as many (E + 1 counts for every 256 picks stand in one array)."""
     return _ops.sort_picks(sel, E)
 
 
