@@ -345,8 +345,9 @@ int nq_combine_bwd(const void* dout, int out_type, const void* y, int type, cons
  *   nq_w4_units   number of units (16 rows x 128 columns) of E matrices N x K
  *   nq_w4_layout  q uint8 [E][N][K / 2] (two columns a byte, the even one in the low half; on an even address), scales [E][N][K / group] of any 16-bit type, zeros uint8
  *                 [E][N][K / group] (0 to 15) or NULL (8) -> planes qw [units][1024] bytes, sc [units][16 * 128 / group] 16-bit, zp likewise bytes (NULL
- *                 without zeros), in the order of nq_w4.cu.  A kernel of the caller's own that writes planes cannot stand directly in front of
- *                 nq_w4_matmul in a stream: planes are read before that kernel's writes are sure to be there
+ *                 without zeros), in the order of nq_w4.cu; qw and sc start on 16 bytes, zp on 8 (groups of 32) or 4.  A kernel of the
+ *                 caller's own that writes planes cannot stand directly in front of nq_w4_matmul in a stream: planes are read before that
+ *                 kernel's writes are sure to be there
  *   nq_w4_matmul  out[r] = W x[r] for x [rows][x_stride >= K] of `type` (NQ_F16 or NQ_BF16; rows start on 16 bytes), out [rows][out_stride >= N] of type
  *                 or NQ_F32.  start NULL: one matrix (E = 1) for all rows.  Else int32 [E + 1] on the device: matrix e for the rows start[e] to
  *                 start[e + 1] - 1 (start[0] = 0), zeros into the rows from start[E] on.  status: int32 [1] on the device, set to 1 if a

@@ -290,6 +290,8 @@ bool w4_shape(int E, int N, int K, int g)
 {
     return E >= 1 && E <= kW4MaxExperts && N >= 1 && K <= kW4MaxColumns && (g == 32 || g == 64 || g == 128) && K >= g && K % g == 0;
 }
+// a copy takes the zero points of two rows in a unit: 8 bytes with groups of 32, 4 with others (of 128: two more rows' with them)
+bool w4_zeros_aligned(const void* zp, int g) { return reinterpret_cast<uintptr_t>(zp) % (g == 32 ? 8 : 4) == 0; }
 int w4_strips(int N) { return (N - 1) / 16 + 1; }
 int w4_chunks(int K) { return (K - 1) / 128 + 1; }
 
@@ -391,6 +393,7 @@ int nq_w4_layout(const void* q, const void* scales, const void* zeros, int E, in
     NQ_REQUIRE(nq::w4_shape(E, N, K, group), "nq_w4_layout: E = %d, N = %d, K = %d, group = %d (32, 64 or 128, a divisor of K)", E, N, K, group);
     NQ_REQUIRE(q && scales && qw && sc && !zeros == !zp && nq::aligned16(qw) && nq::aligned16(sc) && reinterpret_cast<uintptr_t>(q) % 2 == 0,
                "nq_w4_layout: null or unaligned pointer");
+    NQ_REQUIRE(nq::w4_zeros_aligned(zp, group), "nq_w4_layout: zero points start on 8 bytes (groups of 32) or 4");
     const int S = nq::w4_strips(N), C = nq::w4_chunks(K);
     NQ_REQUIRE((int64_t)E * S * C <= 0x7fffffff, "nq_w4_layout: too many units");
     const unsigned units = (unsigned)((int64_t)E * S * C);
@@ -410,6 +413,7 @@ int nq_w4_matmul(const void* x, int type, long long x_stride, const void* qw, co
     if (rows == 0) return NQ_OK;
     NQ_REQUIRE(x && qw && sc && out && status, "nq_w4_matmul: null pointer");
     NQ_REQUIRE(nq::aligned16(x) && x_stride % 8 == 0 && nq::aligned16(qw) && nq::aligned16(sc), "nq_w4_matmul: rows of x and planes start on 16 bytes");
+    NQ_REQUIRE(nq::w4_zeros_aligned(zp, group), "nq_w4_matmul: zero points start on 8 bytes (groups of 32) or 4");
     nq::W4 a{(const uint4*)qw, (const uint16_t*)sc, (const uint8_t*)zp, x, start, out, status, x_stride, out_stride, rows, N, K, E, nq::w4_strips(N), nq::w4_chunks(K),
              out_type, 0, 0, 0, 0, 0, -1, INT_MAX};
     int device;

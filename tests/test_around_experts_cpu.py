@@ -38,3 +38,16 @@ def test_a_sort_of_more_picks_than_its_slices_can_count_is_refused():
     L = capi.lib()
     for T in (2 ** 31 - 1, 2 ** 31 - 255):
         assert refused(L.nq_sort_picks(P, T, 1, 1, None, None, P, P, P, 2 ** 31 - 1, None))
+
+
+@no_device
+@pytest.mark.parametrize("group,needs", [(32, 8), (64, 4), (128, 4)])
+def test_zero_points_off_their_copies_alignment_are_refused(group, needs):
+    """the products copy zero points 8 (groups of 32) or 4 bytes at a time; what suffices goes on to the device that is not there"""
+    L = capi.lib()
+    for zp in range(P, P + 17):
+        fits = zp % needs == 0
+        rc = (L.nq_w4_layout(P, P, P, 2, 64, 256, group, P, P, zp, None),
+              L.nq_w4_matmul(P, capi.NQ_F16, 256, P, P, capi.NQ_F16, zp, P, 4, 2, 64, 256, group, P, capi.NQ_F32, 64, P, None),
+              L.nq_w4_matmul(P, capi.NQ_F16, 256, P, P, capi.NQ_F16, zp, None, 40, 1, 64, 256, group, P, capi.NQ_F32, 64, P, None))
+        assert all(r == (capi.NQ_ERR_CUDA if fits else capi.NQ_ERR_ARG) for r in rc), (zp, rc)
