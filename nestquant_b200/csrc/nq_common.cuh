@@ -5,6 +5,7 @@
 #include <stdio.h>
 
 #include <atomic>
+#include <initializer_list>
 
 #include "../../include/nestquant_b200.h"
 
@@ -64,5 +65,12 @@ inline bool allow_shared(int bytes, int device)
 }
 #endif
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// whether all of them (or NULL) start on whole elements of `size` bytes
+inline bool aligned_to(int size, std::initializer_list<const void*> ptrs)
+{
+    for (const void* p : ptrs)
+        if (reinterpret_cast<uintptr_t>(p) % size) return false;
+    return true;
+}
 
 }  // namespace nq

@@ -307,6 +307,7 @@ int sort_pairs(const int64_t* sel, const void* rw, const int64_t* table, int T, 
     cudaStream_t st = (cudaStream_t)stream;
     if (P == 0) return cudaMemsetAsync(start, 0, sizeof(int32_t) * (E + 2), st) == cudaSuccess ? NQ_OK : fail(NQ_ERR_CUDA, "nq_pf_sort: memset failed");
     NQ_REQUIRE(sel && !rw == !table && !pe == !pt && (pe || !table) && pos && scratch, "nq_pf_sort: null pointer");
+    NQ_REQUIRE(aligned_to(8, {sel, table}) && aligned_to(2, {rw}) && aligned_to(4, {pe, pt, pos, start, hits, scratch}), "nq_pf_sort: pointers are not aligned to the elements");
     const int ints = nq_pf_sort_scratch_ints(P, E);
     NQ_REQUIRE(ints > 0, "nq_pf_sort: counts of %d x %d pairs and %d experts are more than an array can hold", T, topk, E);
     NQ_REQUIRE(scratch_ints >= ints, "nq_pf_sort: scratch needs %d ints", ints);

@@ -411,6 +411,8 @@ int nq_route(const void* logits, int type, long long row_stride, const float* bi
     NQ_REQUIRE(!(score == 1 && bias), "nq_route: a bias goes with sigmoid scores");
     if (T == 0) return NQ_OK;
     NQ_REQUIRE(logits && sel && rw, "nq_route: null pointer");
+    NQ_REQUIRE(nq::aligned_to(nq::type_size(type), {logits}) && nq::aligned_to(4, {bias}) && nq::aligned_to(8, {sel}) && nq::aligned_to(nq::type_size(rw_type), {rw}),
+               "nq_route: pointers are not aligned to the elements");
     nq::by_width<nq::RouteLaunch>(type, E, nq::Route{logits, bias, sel, rw, row_stride, T, E, topk, score, renorm != 0, rw_type, 0, 0, scale}, (cudaStream_t)stream);
     return nq::check_launch("nq_route");
 }
@@ -423,6 +425,8 @@ int nq_route_bwd(const void* logits, int type, long long row_stride, const int64
     NQ_REQUIRE(score == 0 || score == 1, "nq_route_bwd: score %d", score);
     if (T == 0) return NQ_OK;
     NQ_REQUIRE(logits && sel && drw && dlogits, "nq_route_bwd: null pointer");
+    NQ_REQUIRE(nq::aligned_to(nq::type_size(type), {logits, dlogits}) && nq::aligned_to(8, {sel}) && nq::aligned_to(nq::type_size(rw_type), {drw}),
+               "nq_route_bwd: pointers are not aligned to the elements");
     nq::by_width<nq::RouteBwdLaunch>(type, E, nq::RouteBwd{logits, sel, drw, dlogits, row_stride, T, E, topk, score, renorm != 0, rw_type, 0, scale}, (cudaStream_t)stream);
     return nq::check_launch("nq_route_bwd");
 }

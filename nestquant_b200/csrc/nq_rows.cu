@@ -312,11 +312,11 @@ int nq_dispatch(const void* x, int type, long long row_stride, const int32_t* po
     NQ_REQUIRE(nq::rows_sizes(type, T, topk, H) && row_stride >= H, "nq_dispatch: type %d, T = %d, topk = %d, H = %d, row stride %lld", type, T, topk, H, row_stride);
     if (T == 0) return NQ_OK;
     NQ_REQUIRE(x && pos && live && xs, "nq_dispatch: null pointer");
+    NQ_REQUIRE(nq::aligned_to(nq::type_size(type), {x, xs}) && nq::aligned_to(4, {pos, live}), "nq_dispatch: pointers are not aligned to the elements");
     // the widest piece that rows, strides and pointers are whole multiples of
     const size_t size = nq::type_size(type);
     int piece = 16;
     while ((size_t)H * size % piece || (size_t)row_stride * size % piece || reinterpret_cast<uintptr_t>(x) % piece || reinterpret_cast<uintptr_t>(xs) % piece) piece /= 2;
-    NQ_REQUIRE(piece >= (int)size, "nq_dispatch: pointers are not aligned to the elements");
     nq::Rows a{x, xs, pos, live, nullptr, (long long)((size_t)row_stride * size / piece), T, topk, H, 0, (int)((size_t)H * size / piece)};
     unsigned grid;
     if (int e = nq::row_grid(T, a.pieces, &grid, "nq_dispatch")) return e;
@@ -333,6 +333,7 @@ int nq_dispatch_bwd(const void* dxs, int type, const int32_t* pos, const int32_t
     NQ_REQUIRE(nq::rows_sizes(type, T, topk, H), "nq_dispatch_bwd: type %d, T = %d, topk = %d, H = %d", type, T, topk, H);
     if (T == 0) return NQ_OK;
     NQ_REQUIRE(dxs && pos && live && dx, "nq_dispatch_bwd: null pointer");
+    NQ_REQUIRE(nq::aligned_to(nq::type_size(type), {dxs, dx}) && nq::aligned_to(4, {pos, live}), "nq_dispatch_bwd: pointers are not aligned to the elements");
     nq::Rows a{dxs, dx, pos, live, nullptr, 0, T, topk, H, 0, 0};
     cudaStream_t st = (cudaStream_t)stream;
     if (type == NQ_F32) return nq::sum_rows<float, float, false>(a, st, "nq_dispatch_bwd");
@@ -347,6 +348,8 @@ int nq_combine(const void* y, int type, const void* rw, int rw_type, const int32
                "nq_combine: types %d, %d -> %d, T = %d, topk = %d, H = %d", type, rw_type, out_type, T, topk, H);
     if (T == 0) return NQ_OK;
     NQ_REQUIRE(y && rw && pos && live && out, "nq_combine: null pointer");
+    NQ_REQUIRE(nq::aligned_to(nq::type_size(type), {y}) && nq::aligned_to(nq::type_size(rw_type), {rw}) && nq::aligned_to(4, {pos, live}) &&
+               nq::aligned_to(nq::type_size(out_type), {out}), "nq_combine: pointers are not aligned to the elements");
     nq::Rows a{y, out, pos, live, rw, 0, T, topk, H, rw_type, 0};
     cudaStream_t st = (cudaStream_t)stream;
     if (type == NQ_F32) return nq::sum_rows<float, float, true>(a, st, "nq_combine");
@@ -361,6 +364,8 @@ int nq_combine_bwd(const void* dout, int out_type, const void* y, int type, cons
                "nq_combine_bwd: types %d, %d, %d, T = %d, topk = %d, H = %d", out_type, type, rw_type, T, topk, H);
     if (T == 0 || !(dy || drw)) return NQ_OK;
     NQ_REQUIRE(dout && (y || !drw) && rw && pos && live, "nq_combine_bwd: null pointer");
+    NQ_REQUIRE(nq::aligned_to(nq::type_size(type), {y, dy}) && nq::aligned_to(nq::type_size(rw_type), {rw, drw}) && nq::aligned_to(4, {pos, live}) &&
+               nq::aligned_to(nq::type_size(out_type), {dout}), "nq_combine_bwd: pointers are not aligned to the elements");
     nq::CombineBwd a{dout, y, rw, dy, drw, pos, live, T, topk, H, rw_type, 0, 0};
     cudaStream_t st = (cudaStream_t)stream;
     if (type == NQ_F32) return nq::combine_bwd<float, float>(a, st);

@@ -391,7 +391,7 @@ int nq_w4_units(int E, int N, int K, int64_t* units)
 int nq_w4_layout(const void* q, const void* scales, const void* zeros, int E, int N, int K, int group, void* qw, void* sc, void* zp, void* stream)
 {
     NQ_REQUIRE(nq::w4_shape(E, N, K, group), "nq_w4_layout: E = %d, N = %d, K = %d, group = %d (32, 64 or 128, a divisor of K)", E, N, K, group);
-    NQ_REQUIRE(q && scales && qw && sc && !zeros == !zp && nq::aligned16(qw) && nq::aligned16(sc) && reinterpret_cast<uintptr_t>(q) % 2 == 0,
+    NQ_REQUIRE(q && scales && qw && sc && !zeros == !zp && nq::aligned16(qw) && nq::aligned16(sc) && nq::aligned_to(2, {q, scales}),
                "nq_w4_layout: null or unaligned pointer");
     NQ_REQUIRE(nq::w4_zeros_aligned(zp, group), "nq_w4_layout: zero points start on 8 bytes (groups of 32) or 4");
     const int S = nq::w4_strips(N), C = nq::w4_chunks(K);
@@ -413,6 +413,7 @@ int nq_w4_matmul(const void* x, int type, long long x_stride, const void* qw, co
     if (rows == 0) return NQ_OK;
     NQ_REQUIRE(x && qw && sc && out && status, "nq_w4_matmul: null pointer");
     NQ_REQUIRE(nq::aligned16(x) && x_stride % 8 == 0 && nq::aligned16(qw) && nq::aligned16(sc), "nq_w4_matmul: rows of x and planes start on 16 bytes");
+    NQ_REQUIRE(nq::aligned_to(4, {start, status}) && nq::aligned_to(nq::type_size(out_type), {out}), "nq_w4_matmul: pointers are not aligned to the elements");
     NQ_REQUIRE(nq::w4_zeros_aligned(zp, group), "nq_w4_matmul: zero points start on 8 bytes (groups of 32) or 4");
     nq::W4 a{(const uint4*)qw, (const uint16_t*)sc, (const uint8_t*)zp, x, start, out, status, x_stride, out_stride, rows, N, K, E, nq::w4_strips(N), nq::w4_chunks(K),
              out_type, 0, 0, 0, 0, 0, -1, INT_MAX};

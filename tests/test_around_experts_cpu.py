@@ -51,3 +51,31 @@ def test_zero_points_off_their_copies_alignment_are_refused(group, needs):
               L.nq_w4_matmul(P, capi.NQ_F16, 256, P, P, capi.NQ_F16, zp, P, 4, 2, 64, 256, group, P, capi.NQ_F32, 64, P, None),
               L.nq_w4_matmul(P, capi.NQ_F16, 256, P, P, capi.NQ_F16, zp, None, 40, 1, 64, 256, group, P, capi.NQ_F32, 64, P, None))
         assert all(r == (capi.NQ_ERR_CUDA if fits else capi.NQ_ERR_ARG) for r in rc), (zp, rc)
+
+
+ENTRIES = {      # entry point: its arguments, and the element size of each pointer among them
+    "nq_route": (dict(logits=P, type=capi.NQ_F32, row_stride=16, bias=P, T=4, E=16, topk=2, score=0, renorm=1, scale=1.0, sel=P, rw=P, rw_type=capi.NQ_F16, stream=None),
+                 dict(logits=4, bias=4, sel=8, rw=2)),
+    "nq_route_bwd": (dict(logits=P, type=capi.NQ_BF16, row_stride=16, sel=P, drw=P, rw_type=capi.NQ_F32, T=4, E=16, topk=2, score=0, renorm=1, scale=1.0, dlogits=P, stream=None),
+                     dict(logits=2, sel=8, drw=4, dlogits=2)),
+    "nq_sort_picks": (dict(sel=P, T=4, topk=2, E=16, pe=P, pt=P, pos=P, start=P, scratch=P, ints=1 << 20, stream=None), dict(sel=8, pe=4, pt=4, pos=4, start=4, scratch=4)),
+    "nq_dispatch": (dict(x=P, type=capi.NQ_F32, row_stride=64, pos=P, live=P, T=4, topk=2, H=64, xs=P, stream=None), dict(x=4, pos=4, live=4, xs=4)),
+    "nq_dispatch_bwd": (dict(dxs=P, type=capi.NQ_F16, pos=P, live=P, T=4, topk=2, H=64, dx=P, stream=None), dict(dxs=2, pos=4, live=4, dx=2)),
+    "nq_combine": (dict(y=P, type=capi.NQ_F16, rw=P, rw_type=capi.NQ_F32, pos=P, live=P, T=4, topk=2, H=64, out=P, out_type=capi.NQ_F32, stream=None),
+                   dict(y=2, rw=4, pos=4, live=4, out=4)),
+    "nq_combine_bwd": (dict(dout=P, out_type=capi.NQ_F32, y=P, type=capi.NQ_F16, rw=P, rw_type=capi.NQ_F16, pos=P, live=P, T=4, topk=2, H=64, dy=P, drw=P, stream=None),
+                       dict(dout=4, y=2, rw=2, pos=4, live=4, dy=2, drw=2)),
+    "nq_w4_layout": (dict(q=P, scales=P, zeros=P, E=2, N=64, K=256, group=64, qw=P, sc=P, zp=P, stream=None), dict(q=2, scales=2)),
+    "nq_w4_matmul": (dict(x=P, type=capi.NQ_F16, x_stride=256, qw=P, sc=P, sc_type=capi.NQ_F16, zp=P, start=P, rows=4, E=2, N=64, K=256, group=64, out=P, out_type=capi.NQ_F32,
+                          out_stride=64, status=P, stream=None), dict(start=4, out=4, status=4)),
+}
+
+
+@no_device
+@pytest.mark.parametrize("name,pointer,size", [(n, p, s) for n, (_, sizes) in ENTRIES.items() for p, s in sizes.items()])
+def test_addresses_off_their_elements_are_refused(name, pointer, size):
+    """a kernel would fault on them; whole elements further on the call goes on to the device that is not there"""
+    entry, base = getattr(capi.lib(), name), ENTRIES[name][0]
+    for off in range(1, 2 * size + 1):
+        rc = entry(*dict(base, **{pointer: P + off}).values())
+        assert rc == (capi.NQ_ERR_ARG if off % size else capi.NQ_ERR_CUDA), off
