@@ -348,6 +348,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_bwd_kernel(RouteBwd a)
 #pragma unroll
         for (int i = 0; i < PER; ++i) { v[i] = eligible(v[i]) ? expf(v[i] - m) : 0.f; s += v[i]; }
         s = warp_sum(s);
+        if (s == 0.f) s = 1.f;                             // no expert is eligible: every p is 0, as the weights are
         const float p = any ? expf(l - m) / s : 0.f, mean = warp_sum(g * p);
         mine = a.scale * p * (g - mean);
 #pragma unroll
