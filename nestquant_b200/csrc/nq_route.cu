@@ -14,7 +14,8 @@
 // 2^-24 |l|, the power of two by 2^-22 of its value, which the slope s (1 - s) <= min(1/4, e^-|l|) makes 2.2e-8 and 6e-8; the sum rounds by 6e-8 s and
 // the reciprocal is off by 1.2e-7 s; the bias adds 6e-8 |score|.  Two neighbours in the sorted list that are
 // further apart than 6e-7 + 3e-7 |score| are in the right order, and so are equal logits with equal biases; a row with any other
-// neighbours among its first topk + 1 is put in order again in 64 bits (one row of a thousand, with 256 experts).
+// neighbours among its first topk + 1 is put in order again in 64 bits (one row of a thousand, with 256 experts).  Where the last pick and
+// the one behind it are equal, the pair says nothing of what follows, so the last pick is held against every expert of the row.
 //
 // A warp per row; lane i holds the experts [i PER, (i + 1) PER), so that the lowest lane that has the largest key also has the lowest id.  The logits are read once
 // (floor of 16,384 rows of 256: 2.8 us, and as much for the gradient's zeros); bound by instructions: 14 us with a bias (16 with
@@ -136,6 +137,27 @@ __device__ __noinline__ int rank_exactly(const L* row, const float* bias, uint2*
     if (lane < n) found[before].y = e;
     __syncwarp();
     return lane < topk && lane < n ? (int)found[lane].y : -1;
+}
+
+template <class L>
+__device__ __forceinline__ bool equal_experts(const L* row, const float* bias, int a, int b) { return to_float(row[a]) == to_float(row[b]) && bias[a] == bias[b]; }
+
+// Whether the row's picks have to be ranked again, where a lane's pick and the one behind it (e1) may be in the wrong order (doubt): they are not equal, or
+// they are the last pair and an expert of the row is neither equal to the last pick nor apart from it
+template <class L>
+__device__ __noinline__ bool in_doubt(const L* row, const float* bias, int E, int topk, int my_e, int e1, bool doubt)
+{
+    if (__any_sync(0xffffffffu, doubt && !equal_experts(row, bias, my_e, e1))) return true;
+    const int last = __shfl_sync(0xffffffffu, my_e, topk - 1);
+    const float l = to_float(row[last]), b = bias[last], s = quick_sigmoid(l) + b;
+    bool any = false;
+    for (int e = threadIdx.x & 31; e < E; e += 32)
+    {
+        const float l1 = to_float(row[e]), b1 = bias[e], s1 = quick_sigmoid(l1) + b1;
+        const bool apart = fabsf(s - s1) > in_doubt_below(fmaxf(fabsf(s), fabsf(s1)));
+        any |= eligible(l1) && eligible(b1) && !apart && !(l1 == l && b1 == b);
+    }
+    return __any_sync(0xffffffffu, any);
 }
 
 // The `picks` largest keys one by one, whatever they are; pick j to lane j, the last one (picks may be 33) also to next_key, next_e
@@ -281,9 +303,9 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(Route a)
         {
             const float s0 = key_float(my_key), s1 = key_float(k1);
             const bool apart = s0 - s1 > in_doubt_below(fmaxf(fabsf(s0), fabsf(s1)));
-            if (!apart) doubt = !(to_float(row[my_e]) == to_float(row[e1]) && a.bias[my_e] == a.bias[e1]);
+            if (!apart) doubt = lane == a.topk - 1 || !equal_experts(row, a.bias, my_e, e1);
         }
-        if (__any_sync(0xffffffffu, doubt))
+        if (__any_sync(0xffffffffu, doubt) && in_doubt(row, a.bias, a.E, a.topk, my_e, e1, doubt))
             my_e = n <= 32 && picks <= 32 ? rank_exactly(row, a.bias, found[0], n, a.topk) : choose_exactly<L, PER>(row, a.bias, a.E, a.topk);
     }
     const bool any = lane < a.topk && my_e >= 0;

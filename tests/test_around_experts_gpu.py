@@ -4,6 +4,8 @@ import math
 import pytest
 import torch
 
+from .test_routing_gpu import choice
+
 pytestmark = pytest.mark.gpu
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
 
@@ -41,3 +43,37 @@ def test_the_gradient_of_a_row_with_nothing_left_is_zero(E, topk, dtype, score, 
     alone = l.detach()[rest].requires_grad_(True)
     want, = torch.autograd.grad(routing.route(alone, topk, score=score, renorm=renorm, scale=2.5, dtype=F32)[1], alone, drw[rest])
     assert torch.equal(got[rest], want)
+
+
+@pytest.mark.parametrize("topk", [1, 2, 8, 31, 32])
+@pytest.mark.parametrize("E", [40, 64, 256, 700])
+def test_a_tie_at_the_last_pick_does_not_hide_a_better_expert_behind_it(E, topk):
+    """the last pick and the next expert have the same logit and bias, and one behind them a score that only 64 bits tell from theirs"""
+    from nestquant_b200 import routing
+    l, b = torch.full((6, E), -4.0, device="cuda"), torch.zeros(E, device="cuda")
+    b[:topk - 1] = 2 - torch.arange(topk - 1, device="cuda") / 64          # what is ahead of them for sure
+    at = topk - 1
+    l[0, at:at + 3] = torch.tensor([17.0, 17.0, 18.0])
+    l[1, [at, at + 1, E - 1]] = torch.tensor([17.0, 17.0, 17.5], device="cuda")
+    l[2, at:] = 17
+    l[2, E - 1] = 19                                                      # more than a warp has lanes
+    l[3, at:] = 17                                                        # nothing better
+    l[4, at:at + 3] = torch.tensor([17.0, 17.0, 16.5])                    # worse
+    l[5, at:at + 4] = torch.tensor([17.0, 17.0, 18.0, 18.0])              # better ones tie too
+    want = choice(l, b, topk)
+    assert want[:3, -1].tolist() == [at + 2, E - 1, E - 1] and want[3:, -1].tolist() == [at, at, at + 2]
+    for dtype in (F32, BF16, F16):
+        assert torch.equal(routing.route(l.to(dtype), topk, bias=b, dtype=F32)[0].cpu(), want)
+
+
+@pytest.mark.parametrize("E,topk", [(8, 1), (33, 8), (128, 8), (256, 8), (256, 32), (1000, 6)])
+def test_16_bit_logits_whose_sigmoids_are_1_in_32_bits(E, topk):
+    """scores that tie often, at the last pick too, among others that 32 bits cannot tell from them"""
+    from nestquant_b200 import routing
+    g = torch.Generator("cuda").manual_seed(E + topk)
+    l = (15 + torch.randint(0, 24, (300, E), generator=g, device="cuda") / 4).bfloat16()
+    l[::7, : E // 2] = -2
+    b = torch.zeros(E, device="cuda")
+    assert torch.equal(routing.route(l, topk, bias=b)[0].cpu(), choice(l, b, topk))
+    b[::3] = 2.0 ** -26
+    assert torch.equal(routing.route(l, topk, bias=b)[0].cpu(), choice(l, b, topk))
