@@ -43,6 +43,8 @@ void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_
 Tensor strided(const Tensor& t) { return t.numel() == 0 || (t.stride(1) == 1 && t.stride(0) >= t.size(1)) ? t : t.contiguous(); }
 int64_t stride_of(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 bool wants_grad(const Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
+// forward-mode derivatives are not built; without this a dual tensor's would be lost without a word, as if they were 0
+void no_tangent(const Tensor& t, const char* what) { NQ_CHECK(!t._fw_grad(/*level=*/0).defined(), what, ": no forward-mode derivative (unpack the dual tensor)"); }
 // gradients that say so when somebody wants to differentiate them
 variable_list once(variable_list grads)
 {
@@ -101,6 +103,7 @@ std::tuple<Tensor, Tensor> route(const Tensor& logits_, int64_t topk, const std:
     const int64_t E = logits_.size(1);
     type_of(logits_.scalar_type(), "route: logits");
     type_of(dtype, "route: weights");
+    no_tangent(logits_, "route: logits");
     NQ_CHECK(score == "sigmoid" || score == "softmax", "route: score ", score, " (sigmoid, softmax)");
     NQ_CHECK(topk >= 1 && topk <= E && topk <= 32 && E <= 1024, "route: ", topk, " picks of ", E, " experts (to 32 of 1024)");
     NQ_CHECK(logits_.size(0) <= 0x7fffffff, "route: too many tokens");
@@ -110,6 +113,7 @@ std::tuple<Tensor, Tensor> route(const Tensor& logits_, int64_t topk, const std:
         on_gpu(*bias, 1, "route: bias");
         NQ_CHECK(bias->scalar_type() == at::kFloat && bias->size(0) == E && bias->is_contiguous(), "route: bias, expected contiguous fp32 [", E, "]");
         NQ_CHECK(!wants_grad(*bias), "route: the bias has no gradient (detach it)");
+        no_tangent(*bias, "route: bias");
         same_device(logits_, *bias, "route");
     }
     const Tensor logits = strided(logits_);
@@ -195,6 +199,7 @@ Tensor dispatch(const Tensor& x_, const OrderPtr& o)
 {
     on_gpu(x_, 2, "dispatch: x");
     type_of(x_.scalar_type(), "dispatch: x");
+    no_tangent(x_, "dispatch: x");
     NQ_CHECK(x_.size(0) == o->T && x_.size(1) >= 1 && x_.size(1) <= 0x7fffffff, "dispatch: x ", x_.sizes(), ", an order of ", o->T, " tokens");
     same_device(x_, o->buf, "dispatch");
     const Tensor x = strided(x_);
@@ -240,6 +245,8 @@ Tensor combine(const Tensor& y_, const OrderPtr& o, const Tensor& rw_, const c10
     on_gpu(rw_, 2, "combine: rw");
     type_of(y_.scalar_type(), "combine: y");
     type_of(rw_.scalar_type(), "combine: rw");
+    no_tangent(y_, "combine: y");
+    no_tangent(rw_, "combine: rw");
     const at::ScalarType dtype = dtype_.value_or(y_.scalar_type());
     NQ_CHECK(y_.size(0) == o->P() && y_.size(1) >= 1 && y_.size(1) <= 0x7fffffff && rw_.size(0) == o->T && rw_.size(1) == o->topk, "combine: y ", y_.sizes(), ", rw ", rw_.sizes(),
              ", an order of ", o->T, " x ", o->topk, " picks");
@@ -306,6 +313,7 @@ Tensor w4_matmul(const W4Ptr& w, const Tensor& x_, const c10::optional<Tensor>& 
              " columns (x fp16 or bf16, result in x's own type or fp32)");
     same_device(x_, w->qw, "W4: x and the weights");
     NQ_CHECK(!wants_grad(x_), "W4: no gradient (detach x, or call under torch.no_grad)");
+    no_tangent(x_, "W4: x");
     NQ_CHECK(w->experts == start.has_value(), "W4: start goes with one matrix per expert, and only with that");
     if (start)
     {

@@ -7,8 +7,8 @@ needs when it is trained.
     out = routing.combine(experts(xs, order.start), order, rw)    #   weighted sums of the picks' rows
 
 Everything is enqueued on the current stream of the tensors' device without a host sync, can be captured in a CUDA graph, and gives the same
-bits every time.  route, dispatch and combine are differentiable (once) in logits, x, y and rw; a call whose tensors need no gradient does not enter
-autograd.  To capture a backward pass, use torch.autograd.grad, or leaves that no eager graph still holds: the engine joins the stream
+bits every time.  route, dispatch and combine are differentiable (once, in backward mode; dual tensors are refused) in logits, x, y and rw; a call whose tensors
+need no gradient does not enter autograd.  To capture a backward pass, use torch.autograd.grad, or leaves that no eager graph still holds: the engine joins the stream
 on which a leaf's gradient was first accumulated, which a capture forbids.  Errors are NestQuantError, raised before anything is enqueued.
 """
 import torch

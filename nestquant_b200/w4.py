@@ -20,7 +20,7 @@ class W4:
     A call takes x [T,K] (fp16 or bf16) to W x as `dtype` (x's own, or fp32), every product and sum in 32 bits: the only rounding is the result's.
     With one matrix per expert, `start` (int32 [E+1] on the device, as Order.start) says whose rows are whose, start[0] = 0; rows from start[E] on give
     zeros.  Enqueued on the current stream of x's device, no host sync, bitwise repeatable.  There is no gradient: the weights are frozen, and an x that
-    needs one is refused."""
+    needs one, or has a tangent, is refused."""
 
     def __init__(s, q, scales, zeros=None):
         s._planes = p = _ops.w4_planes(q, scales, zeros)

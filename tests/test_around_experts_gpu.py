@@ -77,3 +77,30 @@ def test_16_bit_logits_whose_sigmoids_are_1_in_32_bits(E, topk):
     assert torch.equal(routing.route(l, topk, bias=b)[0].cpu(), choice(l, b, topk))
     b[::3] = 2.0 ** -26
     assert torch.equal(routing.route(l, topk, bias=b)[0].cpu(), choice(l, b, topk))
+
+
+def test_inputs_with_tangents_are_refused():
+    """no forward-mode derivative is built, and none is dropped without a word"""
+    import torch.autograd.forward_ad as ad
+    from nestquant_b200 import routing, w4
+    from nestquant_b200.capi import NestQuantError
+    l, b, x, y, rw = (torch.randn(s, device="cuda") for s in ((6, 16), (16,), (6, 128), (12, 128), (6, 2)))
+    o = routing.sort_picks(routing.route(l, 2)[0], 16)
+    q = torch.randint(0, 256, (32, 64), device="cuda", dtype=torch.uint8)
+    w = w4.W4(q, torch.ones(32, 1, device="cuda", dtype=F16))
+    calls = {
+        "logits": (l, lambda t: routing.route(t, 2)), "bias": (b, lambda t: routing.route(l, 2, bias=t)), "x": (x, lambda t: routing.dispatch(t, o)),
+        "y": (y, lambda t: routing.combine(t, o, rw)), "rw": (rw, lambda t: routing.combine(y, o, t)), "4-bit x": (x.half(), lambda t: w(t)),
+    }
+    for name, (t, call) in calls.items():
+        call(t)
+        with ad.dual_level():
+            for leaf in (t, t.clone().requires_grad_(True)):
+                dual = ad.make_dual(leaf, torch.ones_like(t))
+                with pytest.raises(NestQuantError):
+                    call(dual)
+                with torch.no_grad(), pytest.raises(NestQuantError):
+                    call(dual)
+            call(ad.unpack_dual(dual).primal.detach())
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(call, (t,), (torch.ones_like(t),))
