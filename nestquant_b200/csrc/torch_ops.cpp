@@ -148,6 +148,20 @@ struct Order : torch::CustomClassHolder {
     const int32_t* pos_ptr() const { return buf.data_ptr<int32_t>() + E + 2; }
 };
 using OrderPtr = c10::intrusive_ptr<Order>;
+// An order that a backward pass needs.  start and pos are views that a caller can write to: one that was written to since is no longer what the forward pass went
+// by (torch counts the writes; not to a tensor of inference mode, which cannot be told).
+void keep(AutogradContext* ctx, const OrderPtr& o)
+{
+    ctx->saved_data["order"] = c10::IValue::make_capsule(o);
+    ctx->saved_data["version"] = o->buf.is_inference() ? int64_t(-1) : (int64_t)o->buf._version();
+}
+OrderPtr kept(AutogradContext* ctx, const char* what)
+{
+    const auto o = c10::static_intrusive_pointer_cast<Order>(ctx->saved_data["order"].toCapsule());
+    const int64_t version = ctx->saved_data["version"].toInt();
+    NQ_CHECK(version < 0 || version == (int64_t)o->buf._version(), what, ": the order's start or pos was changed behind the backward pass");
+    return o;
+}
 
 OrderPtr sort_picks(const Tensor& sel_, int64_t E)
 {
@@ -179,13 +193,13 @@ Tensor dispatch_now(const Tensor& x, const Order& o)
 struct Dispatch : torch::autograd::Function<Dispatch> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, OrderPtr o)
     {
-        ctx->saved_data["order"] = c10::IValue::make_capsule(o);
+        keep(ctx, o);
         return dispatch_now(x, *o);
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
-        const auto held = ctx->saved_data["order"].toCapsule();
-        const Order& o = static_cast<const Order&>(*held);
+        const OrderPtr held = kept(ctx, "dispatch backward");
+        const Order& o = *held;
         const Tensor dxs = grads[0].detach().contiguous();
         const c10::cuda::CUDAGuard guard(dxs.device());
         Tensor dx = at::empty({o.T, dxs.size(1)}, dxs.options());
@@ -219,15 +233,15 @@ struct Combine : torch::autograd::Function<Combine> {
     static Tensor forward(AutogradContext* ctx, const Tensor& y, const Tensor& rw, OrderPtr o, at::ScalarType dtype)
     {
         ctx->save_for_backward({y, rw});
-        ctx->saved_data["order"] = c10::IValue::make_capsule(o);
+        keep(ctx, o);
         return combine_now(y, rw, *o, dtype);
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &y = saved[0], &rw = saved[1], dout = grads[0].detach().contiguous();
-        const auto held = ctx->saved_data["order"].toCapsule();
-        const Order& o = static_cast<const Order&>(*held);
+        const OrderPtr held = kept(ctx, "combine backward");
+        const Order& o = *held;
         const c10::cuda::CUDAGuard guard(y.device());
         Tensor dy, drw;
         if (ctx->needs_input_grad(0)) dy = at::empty(y.sizes(), y.options());
@@ -349,7 +363,8 @@ PYBIND11_MODULE(_torch_ops, m)
     });
     py::class_<Order, OrderPtr>(m, "Order",
         "The picks of a call sorted by expert (sort_picks).  int32 tensors on the device: start [E+1], first place of each expert's picks (start[E]: where the\n"
-        "picks without an expert begin); pos [T,topk], place of each pick; expert [P] (E: none) and token [P] of each place, P = T * topk.")
+        "picks without an expert begin); pos [T,topk], place of each pick; expert [P] (E: none) and token [P] of each place, P = T * topk.  start and pos are the\n"
+        "order itself: a backward pass raises if they were written to since the forward pass.")
         .def_readonly("T", &Order::T).def_readonly("topk", &Order::topk).def_readonly("E", &Order::E).def_property_readonly("P", &Order::P)
         .def_property_readonly("start", &Order::start).def_property_readonly("pos", &Order::pos)
         .def_property_readonly("expert", &Order::expert).def_property_readonly("token", &Order::token);

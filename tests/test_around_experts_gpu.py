@@ -104,3 +104,31 @@ def test_inputs_with_tangents_are_refused():
             call(ad.unpack_dual(dual).primal.detach())
         with pytest.raises(RuntimeError):
             torch.func.jvp(call, (t,), (torch.ones_like(t),))
+
+
+@pytest.mark.parametrize("part", ["pos", "start"])
+def test_an_order_that_changed_before_its_backward_pass_is_refused(part):
+    from nestquant_b200 import routing
+    sel = torch.randint(0, 8, (20, 3), generator=torch.Generator("cuda").manual_seed(1), device="cuda")
+    x, y, rw = (torch.randn(s, device="cuda", requires_grad=True) for s in ((20, 16), (60, 16), (20, 3)))
+    def both():
+        o = routing.sort_picks(sel, 8)
+        return o, (routing.dispatch(x, o), x), (routing.combine(y, o, rw), y), (routing.combine(y, o, rw), rw)
+    o, *calls = both()
+    for out, leaf in calls:
+        torch.autograd.grad(out.sum(), leaf)
+    o, *calls = both()
+    if part == "pos":
+        o.pos.copy_(o.pos.flip(0))                             # (a permutation still)
+    else:
+        o.start[-1] -= 1
+    for out, leaf in calls:
+        with pytest.raises(RuntimeError, match="changed"):
+            torch.autograd.grad(out.sum(), leaf)
+    with torch.inference_mode():
+        o = routing.sort_picks(sel, 8)                         # (a tensor without a version)
+    out = routing.dispatch(x, o)
+    for _ in range(2):
+        torch.autograd.grad(out, x, torch.ones_like(out), retain_graph=True)
+    out = routing.dispatch(x, routing.sort_picks(sel, 8)) + 0
+    torch.autograd.grad(out.sum(), x)
