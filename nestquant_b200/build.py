@@ -28,13 +28,20 @@ def nvcc():
 
 
 def _torch_ops(lib, force=False, verbose=False):
-    """nestquant_b200/_torch_ops.so, the torch side of routing.py and w4.py (host code only), linked against the library"""
+    """nestquant_b200/_torch_ops.so, the torch side of routing.py and w4.py (host code only), linked against the library.  Where there is no torch the
+    library stands alone, for hosts that call its C entry points."""
     src = os.path.join(CSRC, "torch_ops.cpp")
     if not force and os.path.exists(OPS) and os.path.getmtime(OPS) >= max(os.path.getmtime(f) for f in (src, os.path.join(os.path.dirname(HERE), "include", "nestquant_b200.h"))):
         return OPS
     import sysconfig
-    import torch
-    from torch.utils import cpp_extension as X
+    try:
+        import torch
+        from torch.utils import cpp_extension as X
+    except ImportError as e:
+        if os.path.exists(OPS):
+            os.remove(OPS)          # older than its source or the header
+        print(f"{OPS} is not built, routing.py and w4.py need it: no torch here ({e})", file=sys.stderr)
+        return None
     inc = X.include_paths("cuda") + [sysconfig.get_paths()["include"]]
     libs = X.library_paths("cuda")
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_EXTENSION_NAME=_torch_ops"]
@@ -75,7 +82,7 @@ def _compile(src, verbose):
 
 
 def build(force=False, verbose=False):
-    """Compile every csrc/*.cu and link the shared library, and the torch module on top of it.  Returns the library's path."""
+    """Compile every csrc/*.cu and link the shared library, and, where there is torch, the torch module on top of it.  Returns the library's path."""
     os.makedirs(OBJ, exist_ok=True)
     if not force and os.path.exists(LIB) and os.path.getmtime(LIB) >= _newest_dep():
         _torch_ops(LIB, force, verbose)
