@@ -132,3 +132,42 @@ def test_an_order_that_changed_before_its_backward_pass_is_refused(part):
         torch.autograd.grad(out, x, torch.ones_like(out), retain_graph=True)
     out = routing.dispatch(x, routing.sort_picks(sel, 8)) + 0
     torch.autograd.grad(out.sum(), x)
+
+
+@pytest.mark.parametrize("T", [2, 8, 16, 40, 64, 150])
+def test_a_rows_bits_do_not_depend_on_the_values_of_other_rows(T):
+    """how a row's sums are cut goes by the call's sizes; with one matrix and with one per expert"""
+    from nestquant_b200 import w4
+    N, K, E, g = 272, 1024, 4, 64
+    gen = torch.Generator("cuda").manual_seed(T)
+    q = torch.randint(0, 256, (E, N, K // 2), generator=gen, device="cuda", dtype=torch.uint8)
+    s = (0.01 * torch.randn(E, N, K // g, generator=gen, device="cuda")).half()
+    start = torch.tensor([0, T // 2, T // 2, T - 1, T], dtype=torch.int32, device="cuda")
+    x, other = (torch.randn(T, K, generator=gen, device="cuda").half() for _ in range(2))
+    for call in (w4.W4(q[0], s[0]), lambda x, dtype: w4.W4(q, s)(x, start=start, dtype=dtype)):
+        y = call(x, dtype=F32)
+        for r in (0, T // 2, T - 1):
+            mixed = other.clone()
+            mixed[r] = x[r]
+            got = call(mixed, dtype=F32)
+            assert torch.equal(got[r], y[r]) and not torch.equal(got, y)
+
+
+@pytest.mark.parametrize("T,topk,E", [(1, 1, 1), (40, 3, 9), (3000, 4, 200), (9000, 8, 300)])
+def test_experts_and_tokens_of_the_sorted_places(T, topk, E):
+    """the arrays that nq_sort_picks writes for callers in other languages, in the form of one launch and in that of three"""
+    from nestquant_b200 import capi, routing
+    g = torch.Generator("cuda").manual_seed(T)
+    sel = torch.randint(-1, E + 1, (T, topk), generator=g, device="cuda")
+    P, L = T * topk, capi.lib()
+    pe, pt, pos = (torch.full((P + 1,), -7, dtype=torch.int32, device="cuda") for _ in range(3))
+    start = torch.full((E + 3,), -7, dtype=torch.int32, device="cuda")
+    ints = L.nq_pf_sort_scratch_ints(P, E)
+    scratch = torch.empty(ints, dtype=torch.int32, device="cuda")
+    capi.check(L.nq_sort_picks(*map(capi.ptr, (sel,)), T, topk, E, *map(capi.ptr, (pe, pt, pos, start, scratch)), ints, capi.current_stream()))
+    o = routing.sort_picks(sel, E)
+    assert torch.equal(pe[:P], o.expert) and torch.equal(pt[:P], o.token) and torch.equal(pos[:P], o.pos.flatten()) and torch.equal(start[:E + 1], o.start)
+    flat = sel.flatten().tolist()
+    order = sorted(range(P), key=lambda i: (flat[i] if 0 <= flat[i] < E else E, i))
+    assert pe[:P].tolist() == [flat[i] if 0 <= flat[i] < E else E for i in order] and pt[:P].tolist() == [i // topk for i in order]
+    assert int(start[E + 1]) == P and all(int(t[-1]) == -7 for t in (pe, pt, pos, start))
