@@ -10,7 +10,8 @@
 // topk independent loads or stores are in flight per thread (predicated loads: behind branches they went one by one, 80 us instead of 67); the gradient of combine
 // has warps per token for the dot products, two, four or eight picks at a time (with places for eight 5,001 x 4 x 1,000 took 11 and 22 us: the registers, and loads
 // under predicates that do not hold).  4,096 tokens x 8 picks x 6,144 bf16, us (floor at the copy's 6.54 TB/s): copy 72 (69), sums 66 (69: part of the rows is
-// still in L2), combine's gradient 140 (131); 5,001 x 4 x 1,000: 7.5, 8.8, 16.9 (7.7, 7.7, 13.8).
+// still in L2), combine's gradient 140 (131); 5,001 x 4 x 1,000: 7.5, 8.8, 16.9 (7.7, 7.7, 13.8).  Weighted sums of eight
+// 16-bit picks at a time spill 12 bytes of registers, nothing else here spills.
 #include <initializer_list>
 #include <type_traits>
 

@@ -13,7 +13,9 @@
 // sums.  What made the difference at 512 rows: one row block of 32 per pass of the other kernel 156; this kernel with eight warps of 128 tokens' sums and the MMAs one by
 // one 35; registers by role and two sums an instruction 30; one vote for a chunk's three barriers 24.6.  In groups of 64: scales that stay where they were loaded and
 // the next barrier looked at behind the products 36.5 -> 33.5; in groups of 32: an accumulator read at once 58 -> 55.  Passes of up to 64 rows: an MMA of 16 columns takes
-// ~56 clocks however few tokens it has, and sixteen warps decode.
+// ~56 clocks however few tokens it has, and sixteen warps decode.  Passes of 64 rows in groups of 64 and 32 spill: 832 threads have 72 registers each, and the sums
+// want more, 16 to 32 bytes with fp16 scales, 194 to 244 with bf16 ones; 64 rows of 4,096 x 6,144 take 11.9 and 14.7, with bf16 scales 14.1 and 17.5 (groups of 128, which
+// do not spill: 10.8 and 11.2).
 // Columns of an item may be split over a cluster; each CTA then adds up a share of the tokens, the others' sums come through distributed shared memory.
 // Every mbarrier wait is bounded (nq_tc.cuh): on time-out the CTA raises status[0], waits for its loads and MMAs in flight and ends.
 #include <stddef.h>

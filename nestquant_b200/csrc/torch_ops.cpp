@@ -1,7 +1,7 @@
 // The torch side of the calls around the routed experts: argument checks, outputs, streams and gradients in front of the C entry points.
 //
 // A call through ctypes and a Python autograd function costs the host 10 to 14 us, a backward pass 100; the kernels of a decode step take 2 to 6.  From here
-// they cost a few and about 40.  Nothing here computes: every function makes its outputs and calls libnestquant_b200.so on the current stream of the
+// a call costs 4.5 to 5.5, forward and backward together 50 to 54, of which torch's engine has most (its own exp and the gradient: 49).  Nothing here computes: every function makes its outputs and calls libnestquant_b200.so on the current stream of the
 // tensors' device.  Errors are thrown as nestquant_b200.capi.NestQuantError before anything is enqueued.
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
