@@ -31,15 +31,16 @@ def _torch_ops(lib, force=False, verbose=False):
     """nestquant_b200/_torch_ops.so, the torch side of routing.py and w4.py (host code only), linked against the library.  Where there is no torch the
     library stands alone, for hosts that call its C entry points."""
     src = os.path.join(CSRC, "torch_ops.cpp")
-    if not force and os.path.exists(OPS) and os.path.getmtime(OPS) >= max(os.path.getmtime(f) for f in (src, os.path.join(os.path.dirname(HERE), "include", "nestquant_b200.h"))):
+    fresh = os.path.exists(OPS) and os.path.getmtime(OPS) >= max(os.path.getmtime(f) for f in (src, os.path.join(os.path.dirname(HERE), "include", "nestquant_b200.h")))
+    if fresh and not force:
         return OPS
     import sysconfig
     try:
         import torch
         from torch.utils import cpp_extension as X
     except ImportError as e:
-        if os.path.exists(OPS):
-            os.remove(OPS)          # older than its source or the header
+        if os.path.exists(OPS) and not fresh:
+            os.remove(OPS)          # (older than its source or the header: not beside a newer library)
         print(f"{OPS} is not built, routing.py and w4.py need it: no torch here ({e})", file=sys.stderr)
         return None
     inc = X.include_paths("cuda") + [sysconfig.get_paths()["include"]]

@@ -30,3 +30,11 @@ def test_the_library_builds_without_torch(tmp_path, stale):
     assert r.returncode == 0, r.stderr[-2000:]
     assert r.stdout.strip() == build.LIB and "torch" in r.stderr and "routing" in r.stderr
     assert not ops.exists()                  # an older module does not stay beside a newer library
+
+
+def test_a_module_that_is_up_to_date_stays(tmp_path):
+    ops = tmp_path / "_torch_ops.so"
+    ops.write_text("of this source")
+    code = CODE.replace("build.build()", "build._torch_ops(build.LIB, force=True)")
+    r = subprocess.run([sys.executable, "-c", code, str(ops)], capture_output=True, text=True, cwd=ROOT, timeout=600)
+    assert r.returncode == 0 and r.stdout.strip() == "None" and ops.exists(), r.stderr[-2000:]
